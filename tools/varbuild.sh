@@ -13,7 +13,7 @@ B=build/obj_var_$(basename $OUT .so)
 mkdir -p $B tools/lat
 make -s -C msccl_amd/csrc -j8
 /opt/rocm/bin/hipcc -std=c++17 -O3 -fPIC -Wall -Wno-unused-parameter -Wno-unused-variable -Wno-unused-result \
-  -Imsccl_amd/csrc -Iinclude --offload-arch=gfx950 -munsafe-fp-atomics -Wshadow -ffp-contract=off \
+  -Imsccl_amd/csrc -Iinclude --offload-arch=gfx950 -munsafe-fp-atomics -Wshadow -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops \
   -DMSCCL_SMALL_ONLY "$@" -Rpass-analysis=kernel-resource-usage -c msccl_amd/csrc/device/kernels_f32.hip -o $B/kernels_f32.o 2> $B/res.txt || { cat $B/res.txt; exit 1; }
 OBJS=$(ls build/obj/*.o build/obj/device/*.o | grep -v kernels_f32.o)
 /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -Wl,--no-undefined -o $OUT $OBJS $B/kernels_f32.o -lpthread

@@ -10,7 +10,7 @@ make -s -C msccl_amd/csrc -j8
 pids=()
 for t in $TYPES; do
   /opt/rocm/bin/hipcc -std=c++17 -O3 -fPIC -Wall -Wno-unused-parameter -Wno-unused-variable -Wno-unused-result \
-    -Imsccl_amd/csrc -Iinclude --offload-arch=gfx950 -munsafe-fp-atomics -Wshadow -ffp-contract=off "$@" \
+    -Imsccl_amd/csrc -Iinclude --offload-arch=gfx950 -munsafe-fp-atomics -Wshadow -ffp-contract=off -Xclang -target-feature -Xclang -packed-fp32-ops "$@" \
     -Rpass-analysis=kernel-resource-usage -c msccl_amd/csrc/device/kernels_$t.hip -o $B/kernels_$t.o 2> $B/res_$t.txt &
   pids+=($!)
 done
