@@ -1,0 +1,60 @@
+// The sum of squares of many tensors (include/msccl_amd_ops.h: mscclAmdSquareSum).
+//
+// Bound by reading each element once.  Products and sums are in 64 bits: the square of a 32-bit value
+// is exact there and cannot overflow, and gfx950's 64-bit FMA rate is several times what the loads can
+// feed.  Workgroups add up strided chunks into one partial sum each; a second launch of one workgroup
+// adds the partial sums in a fixed order, so the result does not depend on timing.
+#include "ops.h"
+
+namespace msccl {
+
+template <class T>
+__global__ void __launch_bounds__(kOpsThreads) squareSumKernel(TensorTable<SumTensor> tab, double* partials) {
+  __shared__ double lds[kOpsThreads / 64];
+  double s = 0.0;
+  for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
+    const uint32_t ti = findTensor(tab.starts, tab.n, c);
+    const uint64_t from = (uint64_t)(c - scalarLoad(tab.starts + ti)) * kOpsChunk;
+    const uint64_t left = scalarLoad(&tab.rows[ti].count) - from;
+    const uint32_t mine = threadIdx.x * kOpsVec;
+    const T* data = (const T*)scalarLoad(&tab.rows[ti].data) + from + mine;
+    f32x8 x;
+    if (left >= kOpsChunk) x = load8(data, 8);
+    else if (left > mine) x = load8(data, left - mine < 8 ? (int)(left - mine) : 8);
+    else continue;
+#pragma unroll
+    for (int i = 0; i < 8; i++) s = fma((double)x[i], (double)x[i], s);
+  }
+  s = blockSum(s, lds);
+  if (threadIdx.x == 0) partials[blockIdx.x] = s;
+}
+
+__global__ void __launch_bounds__(kOpsThreads) sumPartialsKernel(const double* partials, int n, double* out) {
+  __shared__ double lds[kOpsThreads / 64];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kOpsThreads) s += partials[i];
+  s = blockSum(s, lds);
+  if (threadIdx.x == 0) *out = s;
+}
+
+template <class T>
+static int launchSum(const TensorTable<SumTensor>& tab, double* out, double* partials, int blocks, void* stream) {
+  // one workgroup's partial sum is the sum
+  hipLaunchKernelGGL(squareSumKernel<T>, dim3(blocks), dim3(kOpsThreads), 0, (hipStream_t)stream, tab,
+                     blocks == 1 ? out : partials);
+  if (hipGetLastError() != hipSuccess) return 1;
+  if (blocks == 1) return 0;
+  hipLaunchKernelGGL(sumPartialsKernel, dim3(1), dim3(kOpsThreads), 0, (hipStream_t)stream, partials, blocks, out);
+  return hipGetLastError() == hipSuccess ? 0 : 1;
+}
+
+int launchSquareSum(const TensorTable<SumTensor>& tab, int type, double* out, double* partials, int blocks, void* stream) {
+  switch (type) {
+    case 6: return launchSum<_Float16>(tab, out, partials, blocks, stream);
+    case 7: return launchSum<float>(tab, out, partials, blocks, stream);
+    case 9: return launchSum<__bf16>(tab, out, partials, blocks, stream);
+  }
+  return 1;
+}
+
+}  // namespace msccl

@@ -1,0 +1,466 @@
+"""Operators of a training step beside the collectives, on torch tensors (include/msccl_amd_ops.h).
+
+Between ReduceScatter and AllGather: SquareSum, whose result AllReduce sums over the ranks for gradient
+clipping, and AdamW, one step over all of a rank's tensors with its states in 32 or in 8 bits.
+sharded_step makes the whole chain on communicators.  Beside AllToAll: the counts of the tokens each
+expert gets and the experts' balance loss (balance_stats, balance_all_reduce over the ranks,
+balance_loss) with its gradient (balance_backward).
+
+Every call is enqueued on the current torch stream of its tensors' device and returns; nothing waits
+for the device but the creation of a plan.  Calls may be captured into a graph (plans are made before
+the capture, and must outlive the graph, as their tensors must).  Wrong arguments raise ValueError or
+TypeError here, or NcclError from the library.
+"""
+import ctypes
+from typing import Optional, Sequence, Union
+
+import torch
+
+from . import BFLOAT16, FLOAT16, FLOAT32, FLOAT64, INT32, INT64, Comm, NcclError, _check, group, lib
+
+_TYPES = {torch.float32: FLOAT32, torch.float16: FLOAT16, torch.bfloat16: BFLOAT16}
+_INDEX = {torch.int32: INT32, torch.int64: INT64}
+_SCORES = {"softmax": 0, "sigmoid": 1}
+STATE_BLOCK = 256  # elements that share a scale in 8-bit states
+
+
+class _AdamWTensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("master", ctypes.c_void_p),
+                ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
+                ("exp_avg_scale", ctypes.c_void_p), ("exp_avg_sq_scale", ctypes.c_void_p),
+                ("count", ctypes.c_size_t), ("weight_decay", ctypes.c_double), ("lr_scale", ctypes.c_double)]
+
+
+class _Router(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("type", ctypes.c_int), ("tokens", ctypes.c_size_t),
+                ("experts", ctypes.c_size_t), ("logit_stride", ctypes.c_size_t), ("index", ctypes.c_void_p),
+                ("index_type", ctypes.c_int), ("top_k", ctypes.c_size_t), ("index_stride", ctypes.c_size_t),
+                ("valid", ctypes.c_void_p), ("score", ctypes.c_int)]
+
+
+_L = None
+
+
+def _lib():
+    global _L
+    if _L is None:
+        L = lib()
+        vp, i, sz, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_double
+        L.mscclAmdSquareSumBytes.argtypes = [sz]
+        L.mscclAmdSquareSumBytes.restype = sz
+        L.mscclAmdSquareSumCreate.argtypes = [ctypes.POINTER(vp), vp, vp, sz, i, vp, sz, vp]
+        L.mscclAmdSquareSumWorkspace.argtypes = [vp]
+        L.mscclAmdSquareSumWorkspace.restype = sz
+        L.mscclAmdSquareSum.argtypes = [vp, vp, vp, sz, vp]
+        L.mscclAmdSquareSumDestroy.argtypes = [vp]
+        L.mscclAmdAdamWBytes.argtypes = [sz]
+        L.mscclAmdAdamWBytes.restype = sz
+        L.mscclAmdAdamWCreate.argtypes = [ctypes.POINTER(vp), vp, sz, i, i, i, vp, vp, sz, vp]
+        L.mscclAmdAdamWSetGrads.argtypes = [vp, vp, sz, vp]
+        L.mscclAmdAdamWStep.argtypes = [vp, d, vp, d, d, d, d, vp, d, vp]
+        L.mscclAmdAdamWDestroy.argtypes = [vp]
+        L.mscclAmdBalanceWorkspace.argtypes = [sz, sz]
+        L.mscclAmdBalanceWorkspace.restype = sz
+        L.mscclAmdBalanceStats.argtypes = [ctypes.POINTER(_Router), vp, vp, vp, sz, vp]
+        L.mscclAmdBalanceLoss.argtypes = [vp, vp, sz, sz, d, vp, vp]
+        L.mscclAmdBalanceBackward.argtypes = [ctypes.POINTER(_Router), vp, d, vp, vp, sz, i, vp]
+        _L = L
+    return _L
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _on:
+    """Makes `device` the current one if it is not (the launches go to the current device)."""
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _flat(t, what: str, dtypes, device=None, numel: Optional[int] = None) -> None:
+    """A contiguous device tensor of one of `dtypes`, or an exception."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor" % what)
+    if t.device.type != "cuda":
+        raise ValueError("%s must be on a GPU" % what)
+    if t.dtype not in dtypes:
+        raise TypeError("%s: %s is not one of %s" % (what, t.dtype, ", ".join(str(x) for x in dtypes)))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % what)
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s, not %s" % (what, t.device, device))
+    if numel is not None and t.numel() != numel:
+        raise ValueError("%s has %d elements, not %d" % (what, t.numel(), numel))
+
+
+class _Plan:
+    """A plan's handle, its device memory and the tensors whose addresses it holds."""
+    _destroy = ""
+
+    def __init__(self):
+        self.handle = ctypes.c_void_p()
+
+    def _memory(self, device, nbytes: int):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("make the plan before the capture")
+        self.device = device
+        self.table = torch.empty(max(8, nbytes), dtype=torch.uint8, device=device)
+
+    def _ready(self):
+        # the table was written on this stream; the plan may be used on any
+        torch.cuda.current_stream(self.device).synchronize()
+
+    def _live(self):
+        if not self.handle:
+            raise ValueError("the plan is closed")
+
+    def close(self) -> None:
+        """Ends the plan.  The device must be done with its calls."""
+        if self.handle:
+            h, self.handle = self.handle, ctypes.c_void_p()
+            _check(getattr(_lib(), self._destroy)(h), self._destroy)
+        self.table = None
+        self.tensors = None
+
+    def __del__(self):
+        try:
+            if self.handle:  # host memory alone: no device call, whatever the moment
+                getattr(_lib(), self._destroy)(self.handle)
+        except Exception:  # noqa: BLE001
+            pass
+
+
+class SquareSum(_Plan):
+    """The sum of the squares of all elements of `tensors` (one type: float32, float16 or bfloat16; one
+    device; contiguous).  Calling it returns a float64 tensor of one element."""
+    _destroy = "mscclAmdSquareSumDestroy"
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        super().__init__()
+        self.tensors = list(tensors)
+        if not self.tensors:
+            raise ValueError("no tensors")
+        first = self.tensors[0]
+        for i, t in enumerate(self.tensors):
+            _flat(t, "tensor %d" % i, (first.dtype,) if first.dtype in _TYPES else tuple(_TYPES), self.tensors[0].device)
+        n = len(self.tensors)
+        L = _lib()
+        with torch.cuda.device(first.device):
+            self._memory(first.device, L.mscclAmdSquareSumBytes(n))
+            ptrs = (ctypes.c_void_p * n)(*[t.data_ptr() for t in self.tensors])
+            counts = (ctypes.c_size_t * n)(*[t.numel() for t in self.tensors])
+            _check(L.mscclAmdSquareSumCreate(ctypes.byref(self.handle), ptrs, counts, n, _TYPES[first.dtype],
+                                             self.table.data_ptr(), self.table.numel(), _stream(first.device)),
+                   "mscclAmdSquareSumCreate")
+            self._ready()
+        self._scratch = L.mscclAmdSquareSumWorkspace(self.handle)
+
+    def __call__(self, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        self._live()
+        if out is not None:
+            _flat(out, "out", (torch.float64,), self.device, 1)
+        with _on(self.device):
+            # scratch of this call's own: calls on several streams, or in several graphs, do not meet in it
+            scratch = torch.empty(self._scratch // 8 + 1, dtype=torch.float64, device=self.device)
+            if out is None:
+                out = torch.empty(1, dtype=torch.float64, device=self.device)
+            rc = _lib().mscclAmdSquareSum(self.handle, out.data_ptr(), scratch.data_ptr(), self._scratch,
+                                          _stream(self.device))
+        if rc:
+            raise NcclError(rc, "mscclAmdSquareSum")
+        return out
+
+
+def adamw_state(param: torch.Tensor, bits: int = 32):
+    """The state of `param` before its first step: (exp_avg, exp_avg_sq), or with bits=8
+    (exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale), all zeros."""
+    n, dev = param.numel(), param.device
+    if bits == 32:
+        return tuple(torch.zeros(n, dtype=torch.float32, device=dev) for _ in range(2))
+    if bits != 8:
+        raise ValueError("states of %r bits (32 or 8)" % (bits,))
+    return (tuple(torch.zeros(n, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2)) +
+            tuple(torch.zeros(-(-n // STATE_BLOCK), dtype=torch.float32, device=dev) for _ in range(2)))
+
+
+def dequantize_state(code: torch.Tensor, scale: torch.Tensor, second: bool = False) -> torch.Tensor:
+    """The 32-bit values of an 8-bit state (second: of exp_avg_sq, whose codes hold square roots)."""
+    x = code.reshape(-1).float() * scale.repeat_interleave(STATE_BLOCK)[:code.numel()]
+    return x.square() if second else x
+
+
+class AdamW(_Plan):
+    """AdamW over many tensors of one device in one launch.
+
+    params and grads: contiguous, one type each (float32, float16, bfloat16); masters: None, or the
+    weights in float32 (read in place of params, both are written).  exp_avgs, exp_avg_sqs: float32, or
+    torch.float8_e4m3fn with exp_avg_scales and exp_avg_sq_scales, one float32 for each 256 elements of
+    a tensor (the last may be shorter); adamw_state makes them.  step: one int64, the steps taken so far.
+    weight_decay, lr_scale: a number, or one for each tensor.  Tensors may have any size and start
+    anywhere; they must not overlap.  Steps of one plan must be ordered after each other."""
+    _destroy = "mscclAmdAdamWDestroy"
+
+    def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+                 exp_avg_sqs: Sequence[torch.Tensor], step: torch.Tensor, masters: Optional[Sequence[torch.Tensor]] = None,
+                 exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
+                 exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
+                 weight_decay: Union[float, Sequence[float]] = 0.0, lr_scale: Union[float, Sequence[float]] = 1.0):
+        super().__init__()
+        n = len(params)
+        if not n:
+            raise ValueError("no tensors")
+        dev = params[0].device
+        bits = 8 if exp_avgs and exp_avgs[0].dtype == torch.float8_e4m3fn else 32
+        if bits == 8 and (exp_avg_scales is None or exp_avg_sq_scales is None):
+            raise ValueError("8-bit states need their scales")
+        if bits == 32 and (exp_avg_scales is not None or exp_avg_sq_scales is not None):
+            raise ValueError("32-bit states have no scales")
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
+        rates = list(lr_scale) if isinstance(lr_scale, (list, tuple)) else [lr_scale] * n
+        state = (torch.float8_e4m3fn,) if bits == 8 else (torch.float32,)
+        lists = [("params", params, (params[0].dtype,) if params[0].dtype in _TYPES else tuple(_TYPES), 1),
+                 ("grads", grads, tuple(_TYPES), 1), ("masters", masters, (torch.float32,), 1),
+                 ("exp_avgs", exp_avgs, state, 1), ("exp_avg_sqs", exp_avg_sqs, state, 1),
+                 ("exp_avg_scales", exp_avg_scales, (torch.float32,), STATE_BLOCK),
+                 ("exp_avg_sq_scales", exp_avg_sq_scales, (torch.float32,), STATE_BLOCK)]
+        for what, ts, dtypes, per in lists:
+            if ts is None:
+                continue
+            if len(ts) != n:
+                raise ValueError("%d %s for %d tensors" % (len(ts), what, n))
+            for i, t in enumerate(ts):
+                _flat(t, "%s[%d]" % (what, i), dtypes, dev, -(-params[i].numel() // per))
+        if len(decay) != n or len(rates) != n:
+            raise ValueError("weight_decay and lr_scale: a number, or one for each tensor")
+        if any(g.dtype != grads[0].dtype for g in grads):
+            raise TypeError("grads must have one type")
+        _flat(step, "step", (torch.int64,), dev, 1)
+        self.tensors = [list(ts) if ts is not None else None for _, ts, _, _ in lists] + [step]
+        self._grad_type = grads[0].dtype
+        rows = (_AdamWTensor * n)()
+        for i in range(n):
+            r = rows[i]
+            r.param, r.grad, r.master, r.exp_avg, r.exp_avg_sq, r.exp_avg_scale, r.exp_avg_sq_scale = [
+                ts[i].data_ptr() if ts is not None else None for _, ts, _, _ in lists]
+            r.count, r.weight_decay, r.lr_scale = params[i].numel(), float(decay[i]), float(rates[i])
+        L = _lib()
+        with torch.cuda.device(dev):
+            self._memory(dev, L.mscclAmdAdamWBytes(n))
+            _check(L.mscclAmdAdamWCreate(ctypes.byref(self.handle), rows, n, _TYPES[params[0].dtype],
+                                         _TYPES[grads[0].dtype], bits, step.data_ptr(), self.table.data_ptr(),
+                                         self.table.numel(), _stream(dev)), "mscclAmdAdamWCreate")
+            self._ready()
+
+    def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
+        """Other gradient tensors (same sizes and type) for the steps enqueued from now on; the earlier
+        steps must be on the current stream or ordered before it."""
+        self._live()
+        params = self.tensors[0]
+        if len(grads) != len(params):
+            raise ValueError("%d gradients for %d tensors" % (len(grads), len(params)))
+        for i, g in enumerate(grads):
+            _flat(g, "grads[%d]" % i, (self._grad_type,), self.device, params[i].numel())
+        ptrs = (ctypes.c_void_p * len(grads))(*[g.data_ptr() for g in grads])
+        with _on(self.device):
+            _check(_lib().mscclAmdAdamWSetGrads(self.handle, ptrs, len(grads), _stream(self.device)),
+                   "mscclAmdAdamWSetGrads")
+        self.tensors[1] = list(grads)
+
+    def step(self, lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8, grad_scale: float = 1.0,
+             grad_square_sum: Optional[torch.Tensor] = None, max_norm: Optional[float] = None) -> None:
+        """One step (the formulas: mscclAmdAdamWStep).  lr: a number, or a float32 tensor of one element,
+        which a captured step reads at each replay.  grad_scale: a factor on the gradients (one over the
+        ranks that were summed, or over a loss scale).  grad_square_sum: the square sum of the gradients as
+        they are, over all ranks; if it is not finite the step changes nothing.  max_norm: clips to it."""
+        self._live()
+        at = None
+        if isinstance(lr, torch.Tensor):
+            _flat(lr, "lr", (torch.float32,), self.device, 1)
+            at, lr = lr.data_ptr(), 0.0
+        total = None
+        if grad_square_sum is not None:
+            _flat(grad_square_sum, "grad_square_sum", (torch.float64,), self.device, 1)
+            total = grad_square_sum.data_ptr()
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("max_norm must be above zero")
+        with _on(self.device):
+            rc = _lib().mscclAmdAdamWStep(self.handle, lr, at, betas[0], betas[1], eps, grad_scale, total,
+                                          max_norm or 0.0, _stream(self.device))
+        if rc:
+            raise NcclError(rc, "mscclAmdAdamWStep")
+
+
+def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: Sequence[torch.Tensor],
+                 params: Sequence[torch.Tensor], plans: Sequence[AdamW], sums: Sequence[SquareSum],
+                 lr: Union[float, Sequence[torch.Tensor]], betas=(0.9, 0.999), eps: float = 1e-8,
+                 max_norm: Optional[float] = None) -> list:
+    """One data-parallel step with the optimizer's state sharded over the ranks, for the ranks of `comms`
+    that this process holds (lists: one entry for each).  grads[r]: that rank's whole flat gradient, nranks
+    equal blocks; shards[r]: a buffer of one block, which ReduceScatter fills with the sum over ranks and
+    plans[r] and sums[r] read; params[r]: the whole flat weights, whose block number `rank` plans[r]
+    updates and AllGather sends to every rank.  The gradients are averaged over the ranks.  A gradient
+    that is not finite on any rank leaves every rank's weights and state as they were.  Returns the
+    square sums of the summed gradient (one float64 of one element for each; its norm is
+    sqrt(sum) / nranks)."""
+    if not len(comms) == len(grads) == len(shards) == len(params) == len(plans) == len(sums) or not comms:
+        raise ValueError("one gradient, shard, weight buffer, plan and square sum for each communicator")
+    n = comms[0].nranks
+    for r, c in enumerate(comms):
+        block = shards[r].numel()
+        dev = torch.device("cuda", c.device)
+        _flat(shards[r], "shards[%d]" % r, tuple(_TYPES), dev)
+        _flat(grads[r], "grads[%d]" % r, (shards[0].dtype,), dev, n * block)
+        _flat(params[r], "params[%d]" % r, (params[0].dtype,) if params[0].dtype in _TYPES else tuple(_TYPES), dev, n * block)
+        if shards[r].dtype != shards[0].dtype or block != shards[0].numel():
+            raise ValueError("the shards must have one size and type")
+        if plans[r].device != dev or sums[r].device != dev:
+            raise ValueError("plans[%d] or sums[%d] is on another device than its communicator" % (r, r))
+    block, es = shards[0].numel(), params[0].element_size()
+    gt, pt = _TYPES[shards[0].dtype], _TYPES[params[0].dtype]
+    with group():
+        for r, c in enumerate(comms):
+            c.reduce_scatter(grads[r].data_ptr(), shards[r].data_ptr(), block, gt, stream=_stream(shards[r].device))
+    totals = [s() for s in sums]
+    with group():
+        for r, c in enumerate(comms):
+            c.all_reduce(totals[r].data_ptr(), totals[r].data_ptr(), 1, FLOAT64, stream=_stream(totals[r].device))
+    for r, p in enumerate(plans):
+        p.step(lr[r] if isinstance(lr, (list, tuple)) else lr, betas, eps, 1.0 / n, totals[r], max_norm)
+    with group():
+        for r, c in enumerate(comms):
+            base = params[r].data_ptr()
+            c.all_gather(base + c.rank * block * es, base, block, pt, stream=_stream(params[r].device))
+    return totals
+
+
+# ---- balance loss of a router's experts ----------------------------------------------------------
+
+def _router(logits, index, top_k, valid, score) -> _Router:
+    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda":
+        raise ValueError("logits must be a tensor on a GPU")
+    if logits.dim() != 2 or logits.dtype not in _TYPES:
+        raise TypeError("logits must be [tokens, experts] of float32, float16 or bfloat16")
+    t, e = logits.shape
+    if (e > 1 and logits.stride(1) != 1) or (t > 1 and logits.stride(0) < e):
+        raise ValueError("logits: a row's elements must be neighbours, and rows must not overlap")
+    r = _Router()
+    r.logits, r.type, r.tokens, r.experts = logits.data_ptr(), _TYPES[logits.dtype], t, e
+    r.logit_stride = logits.stride(0) if t > 1 else e
+    if index is not None:
+        if not isinstance(index, torch.Tensor) or index.dtype not in _INDEX or index.dim() != 2 or index.shape[0] != t:
+            raise TypeError("index must be [tokens, k] of int32 or int64")
+        top_k = index.shape[1]
+        if index.device != logits.device:
+            raise ValueError("index is on %s, not %s" % (index.device, logits.device))
+        if (top_k > 1 and index.stride(1) != 1) or (t > 1 and index.stride(0) < top_k):
+            raise ValueError("index: a row's elements must be neighbours, and rows must not overlap")
+        r.index, r.index_type = index.data_ptr(), _INDEX[index.dtype]
+        r.index_stride = index.stride(0) if t > 1 else top_k
+    r.top_k = top_k
+    if valid is not None:
+        if not isinstance(valid, torch.Tensor):
+            raise TypeError("valid must be a torch tensor")
+        _flat(valid, "valid", (torch.bool, torch.uint8), logits.device, t)
+        r.valid = valid.data_ptr()
+    if score not in _SCORES:
+        raise ValueError("score %r is not one of %s" % (score, ", ".join(_SCORES)))
+    r.score = _SCORES[score]
+    return r
+
+
+def balance_stats(logits: torch.Tensor, index: torch.Tensor, valid: Optional[torch.Tensor] = None,
+                  score: str = "softmax"):
+    """(counts, probs) of a router's choice: counts int64 [experts + 1], the slots of valid tokens that chose
+    each expert and then the number of valid tokens; probs float32 [experts], the sums over valid tokens of
+    softmax(logits), or with score="sigmoid" of sigmoid(logits) over its row's sum.  index [tokens, k]: the
+    chosen experts (one outside [0, experts) is a dropped slot); valid [tokens]: None, or false for padding."""
+    r = _router(logits, index, 0, valid, score)
+    dev = logits.device
+    L = _lib()
+    with _on(dev):
+        size = L.mscclAmdBalanceWorkspace(r.tokens, r.experts)
+        if not size:
+            raise ValueError("%d tokens over %d experts: at most 2^30 tokens, 1 to 1024 experts" % (r.tokens, r.experts))
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        counts = torch.empty(r.experts + 1, dtype=torch.int64, device=dev)
+        probs = torch.empty(r.experts, dtype=torch.float32, device=dev)
+        rc = L.mscclAmdBalanceStats(ctypes.byref(r), counts.data_ptr(), probs.data_ptr(), scratch.data_ptr(), size,
+                                    _stream(dev))
+    if rc:
+        raise NcclError(rc, "mscclAmdBalanceStats")
+    return counts, probs
+
+
+def balance_all_reduce(comms: Sequence[Comm], counts: Sequence[torch.Tensor], probs: Sequence[torch.Tensor]) -> None:
+    """Sums the statistics of balance_stats over all ranks, in place (lists: one entry for each of `comms`,
+    the ranks that this process holds): the loss and gradients are then those of the whole batch."""
+    if not len(comms) == len(counts) == len(probs) or not comms:
+        raise ValueError("one counts and probs for each communicator")
+    for r, c in enumerate(comms):
+        dev = torch.device("cuda", c.device)
+        _flat(probs[r], "probs[%d]" % r, (torch.float32,), dev, probs[0].numel())
+        _flat(counts[r], "counts[%d]" % r, (torch.int64,), dev, probs[0].numel() + 1)
+    for ts, code in ((counts, INT64), (probs, FLOAT32)):
+        with group():
+            for r, c in enumerate(comms):
+                c.all_reduce(ts[r].data_ptr(), ts[r].data_ptr(), ts[r].numel(), code, stream=_stream(ts[r].device))
+
+
+def balance_loss(counts: torch.Tensor, probs: torch.Tensor, top_k: int, coef: float = 1.0) -> torch.Tensor:
+    """coef * experts / (k N^2) * sum of counts[e] * probs[e] (N valid tokens; 0 for none), float32 of one element."""
+    _flat(probs, "probs", (torch.float32,))
+    _flat(counts, "counts", (torch.int64,), probs.device, probs.numel() + 1)
+    with _on(probs.device):
+        loss = torch.empty(1, dtype=torch.float32, device=probs.device)
+        rc = _lib().mscclAmdBalanceLoss(counts.data_ptr(), probs.data_ptr(), probs.numel(), top_k, coef,
+                                        loss.data_ptr(), _stream(probs.device))
+    if rc:
+        raise NcclError(rc, "mscclAmdBalanceLoss")
+    return loss
+
+
+def balance_backward(logits: torch.Tensor, counts: torch.Tensor, top_k: int, coef: float = 1.0,
+                     grad_output: Optional[torch.Tensor] = None, valid: Optional[torch.Tensor] = None,
+                     score: str = "softmax", out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+    """The gradient of balance_loss at these logits (counts: the loss's own, over all ranks; they carry no
+    gradient), in the type of logits; padded rows get zeros.  grad_output: the loss's own gradient, float32
+    of one element.  out: where to write it; accumulate: it is added to what `out` holds."""
+    r = _router(logits, None, top_k, valid, score)
+    dev = logits.device
+    _flat(counts, "counts", (torch.int64,), dev, r.experts + 1)
+    up = None
+    if grad_output is not None:
+        _flat(grad_output, "grad_output", (torch.float32,), dev, 1)
+        up = grad_output.data_ptr()
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs out")
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+    else:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
+            raise ValueError("out must have the shape, type and device of logits")
+        if (r.experts > 1 and out.stride(1) != 1) or (r.tokens > 1 and out.stride(0) < r.experts):
+            raise ValueError("out: a row's elements must be neighbours, and rows must not overlap")
+    stride = out.stride(0) if r.tokens > 1 else r.experts
+    with _on(dev):
+        rc = _lib().mscclAmdBalanceBackward(ctypes.byref(r), counts.data_ptr(), coef, up, out.data_ptr(), stride,
+                                            int(accumulate), _stream(dev))
+    if rc:
+        raise NcclError(rc, "mscclAmdBalanceBackward")
+    return out
+
+
+__all__ = ["SquareSum", "AdamW", "adamw_state", "dequantize_state", "sharded_step", "balance_stats",
+           "balance_all_reduce", "balance_loss", "balance_backward", "STATE_BLOCK"]
