@@ -36,7 +36,8 @@ size_t mscclAmdSquareSumBytes(size_t n);
 ncclResult_t mscclAmdSquareSumCreate(mscclAmdSquareSum_t* plan, const void* const* data, const size_t* counts, size_t n,
                                      ncclDataType_t type, void* device, size_t deviceBytes, hipStream_t stream);
 
-/* Device bytes of scratch that one call needs (8-byte aligned; not shared by calls that may overlap). */
+/* Device bytes of scratch that one call needs (8-byte aligned; not shared by calls that may overlap);
+ * 0 for a few elements, and the workspace is not looked at. */
 size_t mscclAmdSquareSumWorkspace(mscclAmdSquareSum_t plan);
 
 /* *out = the sum over all tensors of x * x, every product and sum in 64 bits (a bfloat16 or 32-bit
@@ -123,7 +124,8 @@ typedef struct {
   mscclAmdScore_t score;       /* p = softmax(x), or sigmoid(x) over its sum */
 } mscclAmdRouter_t;
 
-/* Scratch bytes of mscclAmdBalanceStats (4-byte aligned; not shared by calls that may overlap). */
+/* Scratch bytes of mscclAmdBalanceStats (4-byte aligned; not shared by calls that may overlap); 0 for
+ * a few tokens, and the workspace is not looked at. */
 size_t mscclAmdBalanceWorkspace(size_t tokens, size_t experts);
 
 /* counts[0..experts): the slots of valid tokens that chose the expert; counts[experts]: the valid

@@ -9,9 +9,12 @@ namespace msccl {
 // ---- shared with the host ------------------------------------------------------------------
 
 constexpr int kOpsThreads = 256;
-constexpr int kOpsVec = 8;                              // elements a lane takes at a time
-constexpr uint32_t kOpsChunk = kOpsThreads * kOpsVec;   // elements of one tensor a workgroup takes at a time
-constexpr int kStateBlock = 256;                        // elements that share a scale in 8-bit states
+constexpr int kStateBlock = 256;     // elements that share a scale in 8-bit states
+// elements of one tensor that a workgroup takes at a time
+constexpr int kAdamEach = 8;         // elements a lane
+constexpr uint32_t kAdamChunk = kOpsThreads * kAdamEach;
+constexpr int kSumVecs = 4;          // 16-byte vectors a lane
+constexpr uint32_t sumChunk(size_t elemSize) { return kOpsThreads * (16 / elemSize) * kSumVecs; }
 
 // rows of the tensor tables; a table is [rows][starts: n + 1 chunk numbers, uint32_t]
 struct SumTensor {
@@ -38,7 +41,7 @@ struct AdamControl {
   float invRoot;     // 1 / sqrt(1 - beta2^t)
   float coef;        // on the gradients
   int skip;
-  int pad;
+  uint32_t arrived;  // workgroups of a one-launch step that have read the step count; 0 between steps
 };
 
 template <class Row>
@@ -89,7 +92,7 @@ int launchTableWrite(void* dst, const void* host, size_t bytes, void* stream);
 int launchGradWrite(AdamTensor* rows, const void* const* grads, size_t n, void* stream);
 int launchSquareSum(const TensorTable<SumTensor>& tab, int type, double* out, double* partials, int blocks, void* stream);
 int launchAdamW(const AdamStepArgs& a, int paramType, int gradType, bool master, int bits, void* stream);
-int balanceBlocks(int64_t tokens, int experts);
+int balanceBlocks(int64_t tokens, int experts);   // workgroups of the statistics; one needs no scratch
 int launchBalanceStats(const BalanceArgs& a, int type, bool index64, bool sigmoid, int blocks, void* stream);
 int launchBalanceLoss(const int64_t* counts, const float* probs, int experts, double scale, float* loss, void* stream);
 int launchBalanceBackward(const BalanceArgs& a, int type, bool sigmoid, bool accumulate, void* stream);
@@ -114,69 +117,132 @@ __device__ __forceinline__ OPS_GLOBAL T* inGlobal(T* p) { return (OPS_GLOBAL T*)
 template <class T>
 __device__ __forceinline__ T scalarLoad(const T* p) { return *(const OPS_CONST T*)p; }
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t opsU32x2 __attribute__((ext_vector_type(2)));
 
-// Eight contiguous elements.  The vector types carry their element's alignment only: gfx950 loads and
+// N contiguous elements.  The vector types carry their element's alignment only: gfx950 loads and
 // stores 16 bytes at any address, so tensors that start anywhere take the same path.
-template <class T>
-struct Vec8;
-template <>
-struct Vec8<float> {
-  typedef float V __attribute__((ext_vector_type(8)));
-  typedef float U __attribute__((ext_vector_type(8), aligned(4)));
+template <class T, int N>
+struct VecOf {
+  typedef T V __attribute__((ext_vector_type(N)));
+  typedef T U __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  typedef float F __attribute__((ext_vector_type(N)));
 };
-template <>
-struct Vec8<__bf16> {
-  typedef __bf16 V __attribute__((ext_vector_type(8)));
-  typedef __bf16 U __attribute__((ext_vector_type(8), aligned(2)));
-};
-template <>
-struct Vec8<_Float16> {
-  typedef _Float16 V __attribute__((ext_vector_type(8)));
-  typedef _Float16 U __attribute__((ext_vector_type(8), aligned(2)));
-};
-typedef opsU32x2 U8x8 __attribute__((aligned(1)));
 
-// n: how many of the eight are there (the rest reads as `fill`)
-template <class T>
-__device__ __forceinline__ f32x8 load8(const T* p, int n, float fill = 0.f) {
-  if (n >= 8) return __builtin_convertvector(*(const OPS_GLOBAL typename Vec8<T>::U*)p, f32x8);
-  f32x8 x;
+template <int N, class T>
+__device__ __forceinline__ typename VecOf<T, N>::V loadVec(const T* p) {
+  return *(const OPS_GLOBAL typename VecOf<T, N>::U*)p;
+}
+
+// What is read once and written once a step streams past the caches' other contents.
+template <int N, class T>
+__device__ __forceinline__ typename VecOf<T, N>::V streamVec(const T* p) {
+  return __builtin_nontemporal_load((const OPS_GLOBAL typename VecOf<T, N>::U*)p);
+}
+
+// n: how many of the N are there (the rest reads as `fill`)
+template <int N, class T>
+__device__ __forceinline__ typename VecOf<T, N>::F loadN(const T* p, int n, float fill = 0.f) {
+  if (n >= N) return __builtin_convertvector(streamVec<N>(p), typename VecOf<T, N>::F);
+  typename VecOf<T, N>::F x;
 #pragma unroll
-  for (int i = 0; i < 8; i++) x[i] = i < n ? (float)inGlobal(p)[i] : fill;
+  for (int i = 0; i < N; i++) x[i] = fill;
+  if (n > 0) {   // the last one again in place of those that are not there: the loads need no branches
+    T y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = inGlobal(p)[i < n ? i : n - 1];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = i < n ? (float)y[i] : fill;
+  }
   return x;
 }
 
 // rounds to nearest, ties to even
-template <class T>
-__device__ __forceinline__ void store8(T* p, f32x8 x, int n) {
-  if (n >= 8) {
-    *(OPS_GLOBAL typename Vec8<T>::U*)p = __builtin_convertvector(x, typename Vec8<T>::V);
+template <int N, class T>
+__device__ __forceinline__ void storeN(T* p, typename VecOf<T, N>::F x, int n) {
+  if (n >= N) {
+    const typename VecOf<T, N>::U y = __builtin_convertvector(x, typename VecOf<T, N>::V);
+    __builtin_nontemporal_store(y, (OPS_GLOBAL typename VecOf<T, N>::U*)p);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; i++)
+  for (int i = 0; i < N; i++)
     if (i < n) inGlobal(p)[i] = (T)x[i];
 }
 
-__device__ __forceinline__ opsU32x2 loadBytes8(const uint8_t* p, int n) {
-  if (n >= 8) return *(const OPS_GLOBAL U8x8*)p;
-  opsU32x2 x = {0, 0};
+// the same of N bytes, four to a word
+template <int N>
+struct BytesOf {
+  typedef uint32_t V __attribute__((ext_vector_type(N / 4)));
+  typedef uint32_t U __attribute__((ext_vector_type(N / 4), aligned(1)));
+};
+
+template <int N>
+__device__ __forceinline__ typename BytesOf<N>::V loadBytes(const uint8_t* p, int n) {
+  if (n >= N) return __builtin_nontemporal_load((const OPS_GLOBAL typename BytesOf<N>::U*)p);
+  typename BytesOf<N>::V x = 0;
+  if (n > 0) {
+    uint8_t y[N];
 #pragma unroll
-  for (int i = 0; i < 8; i++)
-    if (i < n) x[i / 4] |= (uint32_t)inGlobal(p)[i] << (8 * (i % 4));
+    for (int i = 0; i < N; i++) y[i] = inGlobal(p)[i < n ? i : n - 1];
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i / 4] |= i < n ? (uint32_t)y[i] << (8 * (i % 4)) : 0;
+  }
   return x;
 }
 
-__device__ __forceinline__ void storeBytes8(uint8_t* p, opsU32x2 x, int n) {
-  if (n >= 8) {
-    *(OPS_GLOBAL U8x8*)p = x;
+template <int N>
+__device__ __forceinline__ void storeBytes(uint8_t* p, typename BytesOf<N>::V x, int n) {
+  if (n >= N) {
+    const typename BytesOf<N>::U y = x;
+    __builtin_nontemporal_store(y, (OPS_GLOBAL typename BytesOf<N>::U*)p);
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; i++)
+  for (int i = 0; i < N; i++)
     if (i < n) inGlobal(p)[i] = (uint8_t)(x[i / 4] >> (8 * (i % 4)));
+}
+
+// ---- exchanges between lanes -------------------------------------------------------------------
+// combine(x, of the lane's partner) over groups of 2, 4, ... L lanes; every lane of a group ends with
+// the same bits.  All of it in vector instructions (DPP up to 16 lanes, gfx950's row swaps beyond): an
+// exchange through LDS takes a hundred cycles, and a row's maximum and sum are five or six in a row.
+// (The mirrors pair a lane with one of the other half; within a half all lanes hold the same by then.)
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true);
+}
+template <int L, class F>
+__device__ __forceinline__ uint32_t reduceLanes(uint32_t x, F combine) {
+  if constexpr (L >= 2) x = combine(x, dpp<0xB1>(x));     // neighbours: quad_perm 1 0 3 2
+  if constexpr (L >= 4) x = combine(x, dpp<0x4E>(x));     // pairs: quad_perm 2 3 0 1
+  if constexpr (L >= 8) x = combine(x, dpp<0x141>(x));    // mirror of 8
+  if constexpr (L >= 16) x = combine(x, dpp<0x140>(x));   // mirror of 16
+  if constexpr (L >= 32) {
+    const auto y = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = combine(y[0], y[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto y = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = combine(y[0], y[1]);
+  }
+  return x;
+}
+template <int L>
+__device__ __forceinline__ float maxOver(float x) {
+  return __builtin_bit_cast(float, reduceLanes<L>(__builtin_bit_cast(uint32_t, x), [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+  }));
+}
+template <int L>
+__device__ __forceinline__ float sumOver(float x) {
+  return __builtin_bit_cast(float, reduceLanes<L>(__builtin_bit_cast(uint32_t, x), [](uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+  }));
+}
+template <int L>
+__device__ __forceinline__ uint32_t umaxOver(uint32_t x) {
+  return reduceLanes<L>(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
 // The tensor that chunk c of a table lies in: the last row whose first chunk is at most c (empty

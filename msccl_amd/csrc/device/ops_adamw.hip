@@ -5,8 +5,9 @@
 // the step is bound by HBM: 28 bytes an element (32-bit weights, or 16-bit ones with a 32-bit copy, and
 // 32-bit moments), 16 or 10 with the moments in a byte each.  One launch takes every tensor: a workgroup
 // takes 2048-element chunks, and finds the chunk's tensor in the table with one ballot a round.  A lane
-// takes 8 neighbours (16-byte loads of 16-bit types), so that a run of 256 elements that share a scale
-// is half a wave and its largest magnitude is five lane exchanges away.
+// takes twice 4 neighbours, so that a wave's 32-bit loads and stores are whole lines one after the
+// other; with states in 8 bits it takes 8 neighbours at once, so that a run of 256 elements that share
+// a scale is half a wave and its largest magnitude five lane exchanges away.
 #include "ops.h"
 
 namespace msccl {
@@ -54,11 +55,12 @@ int launchGradWrite(AdamTensor* rows, const void* const* grads, size_t n, void* 
 
 // ---- the step ----------------------------------------------------------------------------------
 
-// What every element shares, in 64 bits (1 - b2^t loses its digits in 32 for small t): one thread.
-__global__ void adamwBeginKernel(AdamStepArgs a) {
+// What every element shares, in 64 bits (1 - b2^t loses its digits in 32 for small t), from the step
+// count that *a.step + 1 makes t (or *a.step, where the step is left out).
+__device__ __forceinline__ AdamControl adamwControl(const AdamStepArgs& a, int64_t taken) {
   const double s = a.squareSum ? *a.squareSum : 0.0;
   const bool ok = __builtin_isfinite(s);
-  const int64_t t = *a.step + (ok ? 1 : 0);
+  const int64_t t = taken + 1;
   double p1 = 1.0, p2 = 1.0, q1 = a.beta1, q2 = a.beta2;
   for (uint64_t e = t > 0 ? (uint64_t)t : 0; e; e >>= 1) {   // beta^t by squaring
     if (e & 1) { p1 *= q1; p2 *= q2; }
@@ -70,76 +72,104 @@ __global__ void adamwBeginKernel(AdamStepArgs a) {
     const double clip = a.maxNorm / (a.gradScale * sqrt(s) + 1e-6);
     if (clip < 1.0) c *= clip;
   }
-  const double lr = a.lrDevice ? (double)*a.lrDevice : a.lr;
-  a.ctl->lr = lr;
-  a.ctl->rate = lr / (1.0 - p1);
-  a.ctl->invRoot = (float)(1.0 / sqrt(1.0 - p2));
-  a.ctl->coef = (float)c;
-  a.ctl->skip = !ok;
-  if (ok) *a.step = t;
+  AdamControl r;
+  r.lr = a.lrDevice ? (double)*a.lrDevice : a.lr;
+  r.rate = r.lr / (1.0 - p1);
+  r.invRoot = (float)(1.0 / sqrt(1.0 - p2));
+  r.coef = (float)c;
+  r.skip = !ok;
+  r.arrived = 0;
+  return r;
+}
+
+__global__ void adamwBeginKernel(AdamStepArgs a) {
+  const int64_t taken = *a.step;
+  const AdamControl r = adamwControl(a, taken);
+  a.ctl->lr = r.lr;
+  a.ctl->rate = r.rate;
+  a.ctl->invRoot = r.invRoot;
+  a.ctl->coef = r.coef;
+  a.ctl->skip = r.skip;
+  if (!r.skip) *a.step = taken + 1;
 }
 
 // |x| as an integer orders as |x| does, with infinities and NaN on top: its maximum shows both
 __device__ __forceinline__ uint32_t magnitude(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
 
-__device__ __forceinline__ uint32_t halfWaveMax(uint32_t x) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    const uint32_t y = (uint32_t)__shfl_xor((int)x, d, 32);
-    x = x > y ? x : y;
-  }
-  return x;
-}
-
 constexpr float kFp8Max = 448.f;
 constexpr float kFp8Min = 0.001953125f;   // 2^-9
 
-__device__ __forceinline__ f32x8 decode8(opsU32x2 w, float scale) {
-  f32x8 x;
+template <int N>
+__device__ __forceinline__ typename VecOf<float, N>::F decode(typename BytesOf<N>::V w, float scale) {
+  typename VecOf<float, N>::F x;
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
+  for (int h = 0; h < N / 4; h++) {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], false);
     const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[h], true);
-    x[4 * h] = lo[0];
-    x[4 * h + 1] = lo[1];
-    x[4 * h + 2] = hi[0];
-    x[4 * h + 3] = hi[1];
+    x[4 * h] = lo[0] * scale;
+    x[4 * h + 1] = lo[1] * scale;
+    x[4 * h + 2] = hi[0] * scale;
+    x[4 * h + 3] = hi[1] * scale;
   }
-#pragma unroll
-  for (int i = 0; i < 8; i++) x[i] *= scale;
   return x;
 }
 
-// Codes and scale of a run (half a wave, 8 values a lane).  FLOOR: no value above zero gets code zero.
+// Codes and scale of a run (256 / N lanes, N values each).  FLOOR: no value above zero gets code zero.
 // A rounding to 3 fraction bits is off by at most 2^-4 of the value; values under 2^-10 of the unit
-// (scale) become zero.
-template <bool FLOOR>
-__device__ __forceinline__ opsU32x2 encode8(const f32x8& x, float& scale) {
+// (scale) become zero.  Where a value is not finite the scale is NaN, and the codes say nothing.
+template <int N, bool FLOOR>
+__device__ __forceinline__ typename BytesOf<N>::V encode(const typename VecOf<float, N>::F& x, float& scale) {
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
+  for (int i = 0; i < N; i++) {
     const uint32_t y = magnitude(x[i]);
     top = top > y ? top : y;
   }
-  top = halfWaveMax(top);
+  top = umaxOver<kStateBlock / N>(top);
   const float amax = __builtin_bit_cast(float, top);
-  const bool finite = top < 0x7f800000u;
   // (below 2^-118 the reciprocal would overflow: such a run reads back as zeros)
-  const float inv = finite && amax >= 0x1p-118f ? 1.f / amax * kFp8Max : 0.f;
-  scale = finite ? amax * (1.f / kFp8Max) : __builtin_nanf("");
-  f32x8 y;
+  const float inv = amax >= 0x1p-118f ? 1.f / amax * kFp8Max : 0.f;
+  scale = top < 0x7f800000u ? amax * (1.f / kFp8Max) : __builtin_nanf("");
+  float y[N];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    y[i] = finite ? x[i] * inv : 0.f;
-    if (FLOOR && x[i] > 0.f) y[i] = fmaxf(y[i], kFp8Min);
+  for (int i = 0; i < N; i++) {
+    y[i] = x[i] * inv;
+    if (FLOOR) y[i] = fmaxf(y[i], x[i] > 0.f ? kFp8Min : 0.f);
   }
-  opsU32x2 w;
+  typename BytesOf<N>::V w;
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+  for (int h = 0; h < N / 4; h++) {
+    const int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
     w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], c, true);
   }
   return w;
+}
+
+// Square roots of N values >= 0: one Newton step behind the hardware's estimate, s + (v - s^2) / (2 s), the
+// residual exact by FMA, which leaves the rounding of the last addition.  Where a value of the wave is
+// below 2^-96 (the residual would lose its digits) or not finite, the library's.
+template <int N>
+__device__ __forceinline__ typename VecOf<float, N>::F roots(const typename VecOf<float, N>::F& v) {
+  constexpr uint32_t low = 0x0f800000u, span = 0x7f800000u - low;
+  uint32_t far = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, (float)v[i]) - low;
+    far = far > u ? far : u;
+  }
+  typename VecOf<float, N>::F r;
+  if (__builtin_expect(__ballot(far >= span) != 0, 0)) {
+#pragma unroll
+    for (int i = 0; i < N; i++) r[i] = sqrtf(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float y = __builtin_amdgcn_rsqf(v[i]);
+      const float s = v[i] * y;
+      r[i] = fmaf(fmaf(-s, s, v[i]), 0.5f * y, s);
+    }
+  }
+  return r;
 }
 
 // What a chunk's lanes share.
@@ -154,90 +184,135 @@ struct AdamChunk {
   float coef, invRoot, keep, rate;
 };
 
-// A lane's eight elements from `at` on.  FULL: all are there (so that the loads stand together without
-// branches); else n are.
+// A lane's elements of a chunk that begins at `from`.  FULL: the whole chunk is there (so that the loads
+// stand together without branches); else `left` elements are.
 template <class P, class G, bool MASTER, int BITS, bool FULL>
-__device__ __forceinline__ void adamwEight(const AdamStepArgs& a, const AdamChunk& t, uint64_t at, int some) {
-  const int n = FULL ? 8 : some;
-  const uint64_t run = at / kStateBlock;
-  P* param = (P*)t.param + at;
-  float* master = t.master + at;
-  char* mAt = t.m + at * (BITS / 8);
-  char* vAt = t.v + at * (BITS / 8);
-  const f32x8 g = load8((const G*)t.grad + at, n);
-  f32x8 p = MASTER ? load8(master, n) : load8(param, n);
-  f32x8 m, v, r;
-  if constexpr (BITS == 32) {
-    m = load8((const float*)mAt, n);
-    v = load8((const float*)vAt, n);
-  } else {
-    const opsU32x2 mc = loadBytes8((const uint8_t*)mAt, n), vc = loadBytes8((const uint8_t*)vAt, n);
-    m = decode8(mc, n ? inGlobal(t.mScale)[run] : 0.f);
-    v = decode8(vc, n ? inGlobal(t.vScale)[run] : 0.f);
-    v = v * v;
-  }
+__device__ __forceinline__ void adamwChunk(const AdamStepArgs& a, const AdamChunk& t, uint64_t from, int left) {
+  constexpr int N = BITS == 8 ? 8 : 4;
+  constexpr int J = kAdamEach / N;
+  constexpr int runLanes = kStateBlock / N;
+  typedef typename VecOf<float, N>::F F;
+  F g[J], p[J], m[J], v[J];
+  typename BytesOf<N>::V mc[J], vc[J];
+  float ms[J], vs[J];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float gi = g[i] * t.coef;
-    m[i] = a.b1 * m[i] + a.c1 * gi;
-    v[i] = a.b2 * v[i] + a.c2 * (gi * gi);
-    r[i] = sqrtf(v[i]);
-    p[i] = p[i] * t.keep - t.rate * (m[i] / (r[i] * t.invRoot + a.eps));
-  }
-  if (MASTER) store8(master, p, n);
-  store8(param, p, n);
-  if constexpr (BITS == 32) {
-    store8((float*)mAt, m, n);
-    store8((float*)vAt, v, n);
-  } else {
-    if (!FULL) {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (i >= n) m[i] = r[i] = 0.f;   // behind the tensor's end: no part of the run's scale
+  for (int j = 0; j < J; j++) {
+    const uint32_t mine = (j * kOpsThreads + threadIdx.x) * N;
+    const uint64_t at = from + mine;
+    const int n = FULL ? N : left - (int)mine;
+    g[j] = loadN<N>((const G*)t.grad + at, n);
+    if constexpr (MASTER) p[j] = loadN<N>(t.master + at, n);
+    else p[j] = loadN<N>((const P*)t.param + at, n);
+    if constexpr (BITS == 32) {
+      m[j] = loadN<N>((const float*)t.m + at, n);
+      v[j] = loadN<N>((const float*)t.v + at, n);
+    } else {
+      mc[j] = loadBytes<N>((const uint8_t*)t.m + at, n);
+      vc[j] = loadBytes<N>((const uint8_t*)t.v + at, n);
+      ms[j] = FULL || n > 0 ? inGlobal(t.mScale)[at / kStateBlock] : 0.f;
+      vs[j] = FULL || n > 0 ? inGlobal(t.vScale)[at / kStateBlock] : 0.f;
     }
-    float ms, vs;
-    const opsU32x2 mc = encode8<false>(m, ms), vc = encode8<true>(r, vs);
-    storeBytes8((uint8_t*)mAt, mc, n);
-    storeBytes8((uint8_t*)vAt, vc, n);
-    if (n && (threadIdx.x & 31) == 0) {
-      inGlobal(t.mScale)[run] = ms;
-      inGlobal(t.vScale)[run] = vs;
+  }
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    const uint32_t mine = (j * kOpsThreads + threadIdx.x) * N;
+    const uint64_t at = from + mine;
+    const int n = FULL ? N : left - (int)mine;
+    if constexpr (BITS == 8) {
+      m[j] = decode<N>(mc[j], ms[j]);
+      v[j] = decode<N>(vc[j], vs[j]);
+      v[j] = v[j] * v[j];
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float gi = g[j][i] * t.coef;
+      m[j][i] = a.b1 * m[j][i] + a.c1 * gi;
+      v[j][i] = a.b2 * v[j][i] + a.c2 * (gi * gi);
+    }
+    F r = roots<N>(v[j]);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      // (the reciprocal is within one unit; the denominator is zero or at least 2^-75)
+      const float step = m[j][i] * __builtin_amdgcn_rcpf(fmaf(r[i], t.invRoot, a.eps));
+      p[j][i] = fmaf(-t.rate, step, p[j][i] * t.keep);
+    }
+    if constexpr (MASTER) storeN<N>(t.master + at, p[j], n);
+    storeN<N>((P*)t.param + at, p[j], n);
+    if constexpr (BITS == 32) {
+      storeN<N>((float*)t.m + at, m[j], n);
+      storeN<N>((float*)t.v + at, v[j], n);
+    } else {
+      if (!FULL) {
+#pragma unroll
+        for (int i = 0; i < N; i++)
+          if (i >= n) m[j][i] = r[i] = 0.f;   // behind the tensor's end: no part of the run's scale
+      }
+      const auto mw = encode<N, false>(m[j], ms[j]);
+      const auto vw = encode<N, true>(r, vs[j]);
+      storeBytes<N>((uint8_t*)t.m + at, mw, n);
+      storeBytes<N>((uint8_t*)t.v + at, vw, n);
+      if ((FULL || n > 0) && threadIdx.x % runLanes == 0) {
+        inGlobal(t.mScale)[at / kStateBlock] = ms[j];
+        inGlobal(t.vScale)[at / kStateBlock] = vs[j];
+      }
     }
   }
 }
 
-template <class P, class G, bool MASTER, int BITS>
+// ONE: the step in one launch, every workgroup making what all share by itself.  The last of them to
+// have read the step count advances it.
+template <class P, class G, bool MASTER, int BITS, bool ONE>
 __global__ void __launch_bounds__(kOpsThreads) adamwKernel(AdamStepArgs a) {
-  if (scalarLoad(&a.ctl->skip)) return;
-  const float coef = scalarLoad(&a.ctl->coef), invRoot = scalarLoad(&a.ctl->invRoot);
-  const double lr = scalarLoad(&a.ctl->lr), rate = scalarLoad(&a.ctl->rate);
+  AdamControl ctl;
+  if constexpr (ONE) {
+    const int64_t taken = __hip_atomic_load(a.step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // the count has arrived in this lane before the workgroup says so
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::"v"((uint32_t)taken), "v"((uint32_t)(taken >> 32)) : "memory");
+    __syncthreads();
+    ctl = adamwControl(a, taken);
+    if (threadIdx.x == 0 &&
+        __hip_atomic_fetch_add(&a.ctl->arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1) {
+      __hip_atomic_store(&a.ctl->arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (!ctl.skip) __hip_atomic_store(a.step, taken + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  } else {
+    ctl.skip = scalarLoad(&a.ctl->skip);
+    ctl.coef = scalarLoad(&a.ctl->coef);
+    ctl.invRoot = scalarLoad(&a.ctl->invRoot);
+    ctl.lr = scalarLoad(&a.ctl->lr);
+    ctl.rate = scalarLoad(&a.ctl->rate);
+  }
+  if (ctl.skip) return;
   for (uint32_t c = blockIdx.x; c < a.tab.chunks; c += gridDim.x) {
     const uint32_t ti = findTensor(a.tab.starts, a.tab.n, c);
     const AdamTensor* t = a.tab.rows + ti;
-    const uint64_t from = (uint64_t)(c - scalarLoad(a.tab.starts + ti)) * kOpsChunk;
+    const uint64_t from = (uint64_t)(c - scalarLoad(a.tab.starts + ti)) * kAdamChunk;
     const uint64_t left = scalarLoad(&t->count) - from;
     const double lrScale = scalarLoad(&t->lrScale);
     const AdamChunk k = {scalarLoad(&t->param), scalarLoad(&t->grad), scalarLoad(&t->master), (char*)scalarLoad(&t->m),
-                         (char*)scalarLoad(&t->v), scalarLoad(&t->mScale), scalarLoad(&t->vScale), coef, invRoot,
-                         (float)(1.0 - lr * lrScale * scalarLoad(&t->decay)), (float)(rate * lrScale)};
-    const uint32_t mine = threadIdx.x * kOpsVec;
-    if (left >= kOpsChunk) {
-      adamwEight<P, G, MASTER, BITS, true>(a, k, from + mine, 8);
-    } else {
-      const int n = (int)left - (int)mine;
-      adamwEight<P, G, MASTER, BITS, false>(a, k, from + mine, n < 0 ? 0 : n > 8 ? 8 : n);
-    }
+                         (char*)scalarLoad(&t->v), scalarLoad(&t->mScale), scalarLoad(&t->vScale), ctl.coef, ctl.invRoot,
+                         (float)(1.0 - ctl.lr * lrScale * scalarLoad(&t->decay)), (float)(ctl.rate * lrScale)};
+    if (left >= kAdamChunk) adamwChunk<P, G, MASTER, BITS, true>(a, k, from, 0);
+    else adamwChunk<P, G, MASTER, BITS, false>(a, k, from, (int)left);
   }
 }
+
+// Up to this many workgroups one launch: it saves the first launch's time, and costs each workgroup the
+// shared values' arithmetic and one atomic on one address, which thousands of workgroups would queue for.
+constexpr uint32_t kOneLaunch = 512;
 
 template <class P, class G, bool MASTER, int BITS>
 static int launchStep(const AdamStepArgs& a, void* stream) {
   constexpr uint32_t most = 1u << 20;   // a launch's threads are counted in 32 bits
   const uint32_t grid = a.tab.chunks < most ? a.tab.chunks : most;
+  if (grid && grid <= kOneLaunch) {
+    hipLaunchKernelGGL((adamwKernel<P, G, MASTER, BITS, true>), dim3(grid), dim3(kOpsThreads), 0, (hipStream_t)stream, a);
+    return hipGetLastError() == hipSuccess ? 0 : 1;
+  }
   hipLaunchKernelGGL(adamwBeginKernel, dim3(1), dim3(1), 0, (hipStream_t)stream, a);
   if (hipGetLastError() != hipSuccess) return 1;
   if (grid == 0) return 0;
-  hipLaunchKernelGGL((adamwKernel<P, G, MASTER, BITS>), dim3(grid), dim3(kOpsThreads), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL((adamwKernel<P, G, MASTER, BITS, false>), dim3(grid), dim3(kOpsThreads), 0, (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 

@@ -8,33 +8,16 @@
 // the sums over a row are lane exchanges.  A lane's columns are the same in every row it takes: the
 // sums over rows stay in its registers too, then one exchange through LDS and one partial sum a
 // workgroup, which a second launch adds in a fixed order in 64 bits.  Counts are integers: their
-// atomics (in LDS) give the same result in any order.
+// atomics (in LDS) give the same result in any order.  The statistics' workgroups have 1024 threads:
+// two of them fill a CU, and there are few partial sums to add.
 #include "ops.h"
 
 namespace msccl {
 
-// e^x by 2^x: t = x log2(e) rounded, e = what that rounding and log2(e)'s own left out, e^x = 2^t (1 + e ln 2).
-// For x <= 0 within about one unit of the last place; -inf gives 0.
-__device__ __forceinline__ float expNeg(float x) {
-  constexpr float hi = 1.44269502f, lo = 1.92596303e-8f, ln2 = 0.693147182f;
-  const float t = x * hi;
-  const float y = __builtin_amdgcn_exp2f(t);
-  const float e = fmaf(x, lo, fmaf(x, hi, -t));
-  return x < -87.f ? y : fmaf(y, e * ln2, y);   // (also keeps -inf away from the correction)
-}
-
-template <int LPR>
-__device__ __forceinline__ float rowMax(float x) {
-#pragma unroll
-  for (int d = LPR / 2; d; d >>= 1) x = fmaxf(x, __shfl_xor(x, d));
-  return x;
-}
-template <int LPR>
-__device__ __forceinline__ float rowSum(float x) {
-#pragma unroll
-  for (int d = LPR / 2; d; d >>= 1) x += __shfl_xor(x, d);
-  return x;
-}
+// e^x for x <= 0 as 2^(x log2 e): the product's rounding and the constant's are 1.3 units of 2^-24 times
+// |x| in the result, and the hardware's 2^t is within a unit of the last place.  What is far below the
+// row's maximum, where |x| is large, weighs as little; -inf gives 0.
+__device__ __forceinline__ float expNeg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 
 // The row's unnormalised scores in place of its logits: e^(x - max) or sigmoid(x) (0 outside the row).
 // Returns the lane's part of their sum.  SLOPE: also 1 - sigmoid(x), which 1 - s would round away near 1.
@@ -46,11 +29,12 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
     for (int j = 0; j < VPL; j++)
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        // e = e^-|x|: 1 / (1 + e), or e / (1 + e) left of zero
+        // e = e^-|x|: 1 / (1 + e), or e / (1 + e) left of zero (the reciprocal of 1 to 2: within one unit)
         const float e = expNeg(-fabsf(x[j][i]));
+        const float r = __builtin_amdgcn_rcpf(1.f + e), er = e * r;
         const bool right = x[j][i] >= 0.f;
-        if constexpr (SLOPE) slope[j][i] = (right ? e : 1.f) / (1.f + e);
-        x[j][i] = (right ? 1.f : e) / (1.f + e);
+        if constexpr (SLOPE) slope[j][i] = right ? er : r;
+        x[j][i] = right ? r : er;
         sum += x[j][i];
       }
   } else {
@@ -59,7 +43,7 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
     for (int j = 0; j < VPL; j++)
 #pragma unroll
       for (int i = 0; i < 8; i++) top = fmaxf(top, x[j][i]);
-    top = rowMax<LPR>(top);
+    top = maxOver<LPR>(top);
     // a row of -inf alone has no scores; its sum stays 0
     const float from = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
@@ -73,106 +57,176 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
   return sum;
 }
 
-__device__ __forceinline__ int columns(int experts, int col) {   // of the lane's eight, how many are there
-  const int n = experts - col;
-  return n >= 8 ? 8 : n > 0 ? n : 0;
+// One over the row's sum; 0 for a row without scores.  A softmax's is 1 to 1024, where the hardware's
+// reciprocal is within one unit; a sum of sigmoids may be as small as a 32-bit value gets.
+template <bool SIG>
+__device__ __forceinline__ float inverse(float z) {
+  if constexpr (SIG) return z == 0.f ? 0.f : 1.f / z;
+  else return z == 0.f ? 0.f : __builtin_amdgcn_rcpf(z);
 }
 
-template <class T, int LPR, int VPL, bool SIG, bool IDX64>
-__global__ void __launch_bounds__(kOpsThreads) balanceStatsKernel(BalanceArgs a) {
-  constexpr int rowsPer = kOpsThreads / LPR;
-  constexpr int width = LPR * VPL * 8;
-  constexpr int waves = kOpsThreads / 64;
-  __shared__ uint32_t hist[width + 1];
-  __shared__ float sums[waves][width];
-  for (int i = threadIdx.x; i <= width; i += kOpsThreads) hist[i] = 0;
-  __syncthreads();
-
-  uint32_t here = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kOpsThreads + threadIdx.x; row < a.tokens;
-       row += (int64_t)gridDim.x * kOpsThreads) {
-    if (a.valid && !a.valid[row]) continue;
-    here++;
-    for (int j = 0; j < a.topK; j++) {
-      const int64_t e = IDX64 ? ((const int64_t*)a.index)[row * a.indexStride + j]
-                              : (int64_t)((const int32_t*)a.index)[row * a.indexStride + j];
-      if ((uint64_t)e < (uint64_t)a.experts) atomicAdd(&hist[e], 1u);
-    }
+// A lane's eight columns of a row: base + i for i from `skip` up to `end`.  Where a row's end leaves
+// fewer than eight, the eight before the end, without those that the lane before has: any row of eight
+// or more is read in whole vectors that stay inside it.
+struct Columns {
+  int base, skip, end;
+  bool whole;   // of every lane of the row (the wave's: a scalar)
+  __device__ __forceinline__ Columns(int experts, int width, int col) {
+    base = experts < 8 ? 0 : col < experts - 8 ? col : experts - 8;
+    skip = col - base < 8 ? col - base : 8;
+    end = experts < 8 ? experts : 8;
+    whole = experts % 8 == 0 && experts == width;
   }
-  if (here) atomicAdd(&hist[width], here);
+  __device__ __forceinline__ bool has(int i) const { return i >= skip && i < end; }
+};
+
+// The lane's eight of a row; `none` in the place of columns that are not its own.
+template <class T, int LPR>
+__device__ __forceinline__ f32x8 loadRow(const T* row, const Columns& c, float none) {
+  f32x8 x;
+  if (LPR == 1 && c.end < 8) {
+    T y[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = inGlobal(row)[i < c.end ? i : c.end - 1];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = (float)y[i];
+  } else {
+    x = __builtin_convertvector(loadVec<8>(row + c.base), f32x8);
+  }
+  if (!c.whole) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = c.has(i) ? x[i] : none;
+  }
+  return x;
+}
+
+constexpr int kStatsThreads = 1024;
+
+template <class T, int LPR, int VPL, bool SIG, bool IDX64>
+__global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs a, int64_t rowsEach) {
+  constexpr int rowsPer = kStatsThreads / LPR;
+  constexpr int width = LPR * VPL * 8;
+  constexpr int waves = kStatsThreads / 64;
+  constexpr int copies = width <= 128 ? waves : 1;   // few experts: every wave counts by itself
+  __shared__ uint32_t hist[copies][width];
+  __shared__ uint32_t valid;
+  __shared__ float sums[waves / 2][width];
+  const int wave = threadIdx.x / 64;
+  const int64_t begin = blockIdx.x * rowsEach;
+  const int64_t first = begin < a.tokens ? begin : a.tokens;   // (the last workgroups may have none)
+  const int64_t end = a.tokens - first < rowsEach ? a.tokens : first + rowsEach;
+
+  for (int i = threadIdx.x; i < copies * width; i += kStatsThreads) (&hist[0][0])[i] = 0;
+  if (threadIdx.x == 0) valid = 0;
+  __syncthreads();
+  const uint32_t slots = (uint32_t)(end - first) * (uint32_t)a.topK;
+  for (uint32_t s = threadIdx.x; s < slots; s += kStatsThreads) {
+    const uint32_t r = s / (uint32_t)a.topK;
+    const int64_t row = first + r;
+    const int64_t at = row * a.indexStride + (s - r * (uint32_t)a.topK);
+    const bool here = !a.valid || inGlobal(a.valid)[row];
+    const int64_t e = IDX64 ? inGlobal((const int64_t*)a.index)[at] : (int64_t)inGlobal((const int32_t*)a.index)[at];
+    if (here && (uint64_t)e < (uint64_t)a.experts) atomicAdd(&hist[copies == 1 ? 0 : wave][e], 1u);
+  }
 
   const int lane = threadIdx.x % LPR;
+  const Columns c0(a.experts, width, lane * 8), c1(a.experts, width, (LPR + lane) * 8);
+  const float none = -__builtin_inff();
   f32x8 acc[VPL];
 #pragma unroll
   for (int j = 0; j < VPL; j++) acc[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};
-  for (int64_t row = (int64_t)blockIdx.x * rowsPer + threadIdx.x / LPR; row < a.tokens;
-       row += (int64_t)gridDim.x * rowsPer) {
-    if (a.valid && !a.valid[row]) continue;
+  uint32_t here = 0;
+  for (int64_t row = first + threadIdx.x / LPR; row < end; row += rowsPer) {
+    if (a.valid && !inGlobal(a.valid)[row]) continue;
+    here++;
+    const T* at = (const T*)a.logits + row * a.logitStride;
     f32x8 x[VPL];
-#pragma unroll
-    for (int j = 0; j < VPL; j++) {
-      const int col = (j * LPR + lane) * 8;
-      x[j] = load8((const T*)a.logits + row * a.logitStride + col, columns(a.experts, col), -__builtin_inff());
-    }
-    const float z = rowSum<LPR>(scores<LPR, VPL, SIG, false>(x, nullptr));
-    const float inv = z == 0.f ? 0.f : 1.f / z;
+    x[0] = loadRow<T, LPR>(at, c0, none);
+    if constexpr (VPL == 2) x[1] = loadRow<T, LPR>(at, c1, none);
+    const float z = sumOver<LPR>(scores<LPR, VPL, SIG, false>(x, nullptr));
+    const float inv = inverse<SIG>(z);
 #pragma unroll
     for (int j = 0; j < VPL; j++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) acc[j][i] += x[j][i] * inv;
+      for (int i = 0; i < 8; i++) acc[j][i] = fmaf(x[j][i], inv, acc[j][i]);
   }
-  // over the wave's rows, then over the waves
+  if (here && lane == 0) atomicAdd(&valid, here);
+  // over the wave's rows, then over the waves: the upper half's on top of the lower half's
 #pragma unroll
-  for (int j = 0; j < VPL; j++) {
+  for (int half = 1; half >= 0; half--) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      float s = acc[j][i];
+    for (int j = 0; j < VPL; j++) {
+      const Columns& c = j ? c1 : c0;
 #pragma unroll
-      for (int d = 32; d >= LPR; d >>= 1) s += __shfl_xor(s, d);
-      if ((threadIdx.x & 63) < LPR) sums[threadIdx.x / 64][(j * LPR + lane) * 8 + i] = s;
+      for (int i = 0; i < 8; i++) {
+        if (half) {
+#pragma unroll
+          for (int d = 32; d >= LPR; d >>= 1) acc[j][i] += __shfl_xor(acc[j][i], d);
+        }
+        if ((threadIdx.x & 63) < LPR && wave / (waves / 2) == half && c.has(i)) {
+          float* s = &sums[wave % (waves / 2)][c.base + i];
+          *s = half ? acc[j][i] : *s + acc[j][i];
+        }
+      }
     }
+    __syncthreads();
   }
-  __syncthreads();
   const bool only = gridDim.x == 1;
-  for (int e = threadIdx.x; e < a.experts; e += kOpsThreads) {
+  for (int e = threadIdx.x; e < a.experts; e += kStatsThreads) {
     float s = sums[0][e];
 #pragma unroll
-    for (int w = 1; w < waves; w++) s += sums[w][e];
+    for (int w = 1; w < waves / 2; w++) s += sums[w][e];
+    uint32_t n = hist[0][e];
+#pragma unroll
+    for (int w = 1; w < copies; w++) n += hist[w][e];
     if (only) {
       a.probs[e] = s;
-      a.counts[e] = hist[e];
+      a.counts[e] = n;
     } else {
       a.probPart[(size_t)blockIdx.x * a.experts + e] = s;
-      a.countPart[(size_t)blockIdx.x * (a.experts + 1) + e] = hist[e];
+      a.countPart[(size_t)blockIdx.x * (a.experts + 1) + e] = n;
     }
   }
   if (threadIdx.x == 0) {
-    if (only) a.counts[a.experts] = hist[width];
-    else a.countPart[(size_t)blockIdx.x * (a.experts + 1) + a.experts] = hist[width];
+    if (only) a.counts[a.experts] = valid;
+    else a.countPart[(size_t)blockIdx.x * (a.experts + 1) + a.experts] = valid;
   }
 }
 
-// 16 columns a workgroup, 16 threads down each
-__global__ void __launch_bounds__(kOpsThreads) balanceFinishKernel(BalanceArgs a, int blocks) {
-  __shared__ double ps[kOpsThreads];
-  __shared__ int64_t cs[kOpsThreads];
-  const int e = blockIdx.x * 16 + threadIdx.x % 16;
-  double p = 0.0;
-  int64_t c = 0;
-  for (int b = threadIdx.x / 16; b < blocks; b += 16) {
-    if (e < a.experts) p += (double)a.probPart[(size_t)b * a.experts + e];
-    if (e <= a.experts) c += (int64_t)a.countPart[(size_t)b * (a.experts + 1) + e];
+// The partial sums of at most kStatsBlocks workgroups: 32 columns a workgroup, 32 threads down each, all
+// loads of a thread under way at once.
+constexpr int kStatsBlocks = 512;
+
+__global__ void __launch_bounds__(1024) balanceFinishKernel(BalanceArgs a, int blocks) {
+  __shared__ double ps[32][32];
+  __shared__ int64_t cs[32][32];
+  const int col = threadIdx.x % 32, slice = threadIdx.x / 32;
+  const int e = blockIdx.x * 32 + col;
+  float p[kStatsBlocks / 32];
+  uint32_t c[kStatsBlocks / 32];
+#pragma unroll
+  for (int k = 0; k < kStatsBlocks / 32; k++) {
+    const int b = k * 32 + slice;
+    p[k] = b < blocks && e < a.experts ? a.probPart[(size_t)b * a.experts + e] : 0.f;
+    c[k] = b < blocks && e <= a.experts ? a.countPart[(size_t)b * (a.experts + 1) + e] : 0;
   }
-  ps[threadIdx.x] = p;
-  cs[threadIdx.x] = c;
+  double ps0 = 0.0;
+  int64_t cs0 = 0;
+#pragma unroll
+  for (int k = 0; k < kStatsBlocks / 32; k++) {
+    ps0 += (double)p[k];
+    cs0 += (int64_t)c[k];
+  }
+  ps[slice][col] = ps0;
+  cs[slice][col] = cs0;
   __syncthreads();
-  if (threadIdx.x < 16) {
-    for (int k = 1; k < 16; k++) {
-      p += ps[threadIdx.x + 16 * k];
-      c += cs[threadIdx.x + 16 * k];
+  if (threadIdx.x < 32 && e <= a.experts) {
+    for (int k = 1; k < 32; k++) {
+      ps0 += ps[k][col];
+      cs0 += cs[k][col];
     }
-    if (e < a.experts) a.probs[e] = (float)p;
-    if (e <= a.experts) a.counts[e] = c;
+    if (e < a.experts) a.probs[e] = (float)ps0;
+    a.counts[e] = cs0;
   }
 }
 
@@ -192,6 +246,8 @@ template <class T, int LPR, int VPL, bool SIG, bool ACC>
 __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs a) {
   constexpr int rowsPer = kOpsThreads / LPR;
   const int lane = threadIdx.x % LPR;
+  constexpr int width = LPR * VPL * 8;
+  const Columns c0(a.experts, width, lane * 8), c1(a.experts, width, (LPR + lane) * 8);
   const double n = (double)a.countsIn[a.experts];
   // Every weight less c E / (k N^2) times the mean count of a routing that drops nothing, k N / E: p sums
   // to 1, so the gradient is the same, and with weights that are nearly equal nothing cancels in 32 bits.
@@ -199,39 +255,36 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
   const double up = n > 0 ? a.scale / (n * n) * (a.gradLoss ? (double)*a.gradLoss : 1.0) : 0.0;
   f32x8 w[VPL];
 #pragma unroll
-  for (int j = 0; j < VPL; j++)
+  for (int j = 0; j < VPL; j++) {
+    const Columns& c = j ? c1 : c0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int e = (j * LPR + lane) * 8 + i;
-      w[j][i] = e < a.experts ? (float)(((double)a.countsIn[e] - mean) * up) : 0.f;
-    }
+    for (int i = 0; i < 8; i++) w[j][i] = c.has(i) ? (float)(((double)a.countsIn[c.base + i] - mean) * up) : 0.f;
+  }
   for (int64_t row = (int64_t)blockIdx.x * rowsPer + threadIdx.x / LPR; row < a.tokens;
        row += (int64_t)gridDim.x * rowsPer) {
-    const bool valid = !a.valid || a.valid[row];
+    const bool valid = !a.valid || inGlobal(a.valid)[row];
     if (ACC && !valid) continue;
+    const T* in = (const T*)a.logits + row * a.logitStride;
+    T* out = (T*)a.grad + row * a.gradStride;
     f32x8 x[VPL], slope[VPL];
     if (valid) {
-#pragma unroll
-      for (int j = 0; j < VPL; j++) {
-        const int col = (j * LPR + lane) * 8;
-        x[j] = load8((const T*)a.logits + row * a.logitStride + col, columns(a.experts, col), -__builtin_inff());
-      }
+      x[0] = loadRow<T, LPR>(in, c0, -__builtin_inff());
+      if constexpr (VPL == 2) x[1] = loadRow<T, LPR>(in, c1, -__builtin_inff());
       const float mine = scores<LPR, VPL, SIG, SIG>(x, slope);
       float dot = 0.f;
 #pragma unroll
       for (int j = 0; j < VPL; j++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) dot += x[j][i] * w[j][i];
-      const float z = rowSum<LPR>(mine);
-      dot = rowSum<LPR>(dot);
-      const float inv = z == 0.f ? 0.f : 1.f / z;
+        for (int i = 0; i < 8; i++) dot = fmaf(x[j][i], w[j][i], dot);
+      const float z = sumOver<LPR>(mine);
+      dot = sumOver<LPR>(dot);
+      const float inv = inverse<SIG>(z);
       dot *= inv;
 #pragma unroll
       for (int j = 0; j < VPL; j++)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          const float s = x[j][i];
-          float d = s * inv * (w[j][i] - dot);
+          float d = x[j][i] * inv * (w[j][i] - dot);
           if constexpr (SIG) d *= slope[j][i];
           x[j][i] = d;
         }
@@ -241,11 +294,15 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
     }
 #pragma unroll
     for (int j = 0; j < VPL; j++) {
-      const int col = (j * LPR + lane) * 8;
-      const int k = columns(a.experts, col);
-      T* out = (T*)a.grad + row * a.gradStride + col;
-      if constexpr (ACC) x[j] += load8(out, k);
-      store8(out, x[j], k);
+      const Columns& c = j ? c1 : c0;
+      if constexpr (ACC) x[j] += loadRow<T, LPR>(out, c, 0.f);
+      if (c.whole || (c.skip == 0 && c.end == 8)) {
+        storeN<8>(out + c.base, x[j], 8);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (c.has(i)) inGlobal(out)[c.base + i] = (T)x[j][i];
+      }
     }
   }
 }
@@ -259,10 +316,10 @@ static int lanesPerRow(int experts) {
 }
 
 int balanceBlocks(int64_t tokens, int experts) {
-  const int64_t rowsPer = kOpsThreads / lanesPerRow(experts);
+  const int64_t rowsPer = kStatsThreads / lanesPerRow(experts);
   const int64_t passes = (tokens + rowsPer - 1) / rowsPer;
-  if (passes <= 4) return 1;
-  return (int)(passes < 512 ? passes : 512);
+  if (passes <= 1) return 1;
+  return (int)(passes < kStatsBlocks ? passes : kStatsBlocks);
 }
 
 template <template <int, int> class F, class... A>
@@ -284,13 +341,14 @@ struct Stats {
   template <int LPR, int VPL>
   struct Of {
     static int run(const BalanceArgs* a, bool index64, bool sigmoid, int blocks, hipStream_t s) {
-      const dim3 g(blocks), b(kOpsThreads);
+      const dim3 g(blocks), b(kStatsThreads);
+      const int64_t each = (a->tokens + blocks - 1) / blocks;
       if (sigmoid) {
-        if (index64) hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, true, true>), g, b, 0, s, *a);
-        else hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, true, false>), g, b, 0, s, *a);
+        if (index64) hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, true, true>), g, b, 0, s, *a, each);
+        else hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, true, false>), g, b, 0, s, *a, each);
       } else {
-        if (index64) hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, false, true>), g, b, 0, s, *a);
-        else hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, false, false>), g, b, 0, s, *a);
+        if (index64) hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, false, true>), g, b, 0, s, *a, each);
+        else hipLaunchKernelGGL((balanceStatsKernel<T, LPR, VPL, false, false>), g, b, 0, s, *a, each);
       }
       return hipGetLastError() == hipSuccess ? 0 : 1;
     }
@@ -304,7 +362,7 @@ struct Backward {
     static int run(const BalanceArgs* a, bool sigmoid, bool accumulate, hipStream_t s) {
       constexpr int64_t rowsPer = kOpsThreads / LPR;
       const int64_t passes = (a->tokens + rowsPer - 1) / rowsPer;
-      const dim3 g((uint32_t)(passes < 4096 ? passes : 4096)), b(kOpsThreads);
+      const dim3 g((uint32_t)(passes < 2048 ? passes : 2048)), b(kOpsThreads);
       if (sigmoid) {
         if (accumulate) hipLaunchKernelGGL((balanceBackwardKernel<T, LPR, VPL, true, true>), g, b, 0, s, *a);
         else hipLaunchKernelGGL((balanceBackwardKernel<T, LPR, VPL, true, false>), g, b, 0, s, *a);
@@ -326,7 +384,7 @@ int launchBalanceStats(const BalanceArgs& a, int type, bool index64, bool sigmoi
     case 9: r = pick<Stats<__bf16>::template Of>(a.experts, &a, index64, sigmoid, blocks, s); break;
   }
   if (r != 0 || blocks == 1) return r;
-  hipLaunchKernelGGL(balanceFinishKernel, dim3((a.experts + 1 + 15) / 16), dim3(kOpsThreads), 0, s, a, blocks);
+  hipLaunchKernelGGL(balanceFinishKernel, dim3((a.experts + 1 + 31) / 32), dim3(1024), 0, s, a, blocks);
   return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 

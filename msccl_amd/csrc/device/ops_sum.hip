@@ -11,28 +11,42 @@ namespace msccl {
 template <class T>
 __global__ void __launch_bounds__(kOpsThreads) squareSumKernel(TensorTable<SumTensor> tab, double* partials) {
   __shared__ double lds[kOpsThreads / 64];
+  constexpr int N = 16 / sizeof(T);
+  constexpr uint32_t chunk = sumChunk(sizeof(T));
   double s = 0.0;
   for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
     const uint32_t ti = findTensor(tab.starts, tab.n, c);
-    const uint64_t from = (uint64_t)(c - scalarLoad(tab.starts + ti)) * kOpsChunk;
+    const uint64_t from = (uint64_t)(c - scalarLoad(tab.starts + ti)) * chunk;
     const uint64_t left = scalarLoad(&tab.rows[ti].count) - from;
-    const uint32_t mine = threadIdx.x * kOpsVec;
-    const T* data = (const T*)scalarLoad(&tab.rows[ti].data) + from + mine;
-    f32x8 x;
-    if (left >= kOpsChunk) x = load8(data, 8);
-    else if (left > mine) x = load8(data, left - mine < 8 ? (int)(left - mine) : 8);
-    else continue;
+    const T* data = (const T*)scalarLoad(&tab.rows[ti].data) + from;
+    typename VecOf<T, N>::F x[kSumVecs];
+    if (left >= chunk) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) s = fma((double)x[i], (double)x[i], s);
+      for (int j = 0; j < kSumVecs; j++) x[j] = loadN<N>(data + (j * kOpsThreads + threadIdx.x) * N, N);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kSumVecs; j++) {
+        const uint32_t mine = (j * kOpsThreads + threadIdx.x) * N;
+        x[j] = loadN<N>(data + mine, (int)left - (int)mine);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kSumVecs; j++)
+#pragma unroll
+      for (int i = 0; i < N; i++) s = fma((double)x[j][i], (double)x[j][i], s);
   }
   s = blockSum(s, lds);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-__global__ void __launch_bounds__(kOpsThreads) sumPartialsKernel(const double* partials, int n, double* out) {
-  __shared__ double lds[kOpsThreads / 64];
+__global__ void __launch_bounds__(1024) sumPartialsKernel(const double* partials, int n, double* out) {
+  __shared__ double lds[16];
   double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += kOpsThreads) s += partials[i];
+#pragma unroll
+  for (int k = 0; k < kSumBlocks / 1024; k++) {
+    const int i = k * 1024 + threadIdx.x;
+    s += i < n ? partials[i] : 0.0;
+  }
   s = blockSum(s, lds);
   if (threadIdx.x == 0) *out = s;
 }
@@ -44,7 +58,7 @@ static int launchSum(const TensorTable<SumTensor>& tab, double* out, double* par
                      blocks == 1 ? out : partials);
   if (hipGetLastError() != hipSuccess) return 1;
   if (blocks == 1) return 0;
-  hipLaunchKernelGGL(sumPartialsKernel, dim3(1), dim3(kOpsThreads), 0, (hipStream_t)stream, partials, blocks, out);
+  hipLaunchKernelGGL(sumPartialsKernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, partials, blocks, out);
   return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 

@@ -38,7 +38,7 @@ size_t tableBytes(size_t n) {
 
 // the host image of a table; false: more chunks than 32 bits count
 template <class Row>
-bool makeTable(std::vector<uint64_t>* image, const Row* rows, size_t n, uint32_t* chunks) {
+bool makeTable(std::vector<uint64_t>* image, const Row* rows, size_t n, uint32_t chunk, uint32_t* chunks) {
   image->assign(tableBytes<Row>(n) / 8, 0);
   char* at = (char*)image->data();
   if (n) memcpy(at, rows, n * sizeof(Row));
@@ -46,7 +46,7 @@ bool makeTable(std::vector<uint64_t>* image, const Row* rows, size_t n, uint32_t
   uint64_t c = 0;
   for (size_t i = 0; i < n; i++) {
     starts[i] = (uint32_t)c;
-    c += rows[i].count / kOpsChunk + (rows[i].count % kOpsChunk != 0);
+    c += rows[i].count / chunk + (rows[i].count % chunk != 0);
     if (c > 0x7fffffffull) return false;
   }
   starts[n] = (uint32_t)c;
@@ -107,7 +107,7 @@ ncclResult_t mscclAmdSquareSumCreate(mscclAmdSquareSum_t* plan, const void* cons
     }
     std::vector<uint64_t> image;
     uint32_t chunks;
-    if (!makeTable(&image, rows.data(), n, &chunks)) REFUSE("%s : too many elements", name);
+    if (!makeTable(&image, rows.data(), n, sumChunk(es), &chunks)) REFUSE("%s : too many elements", name);
     if (launchTableWrite(device, image.data(), image.size() * 8, stream)) {
       WARN("%s : launch failed", name);
       return ncclUnhandledCudaError;
@@ -121,8 +121,10 @@ ncclResult_t mscclAmdSquareSumCreate(mscclAmdSquareSum_t* plan, const void* cons
   return ncclSuccess;
 }
 
+static size_t sumScratch(const mscclAmdSquareSumPlan* plan) { return plan->blocks == 1 ? 0 : plan->blocks * sizeof(double); }
+
 size_t mscclAmdSquareSumWorkspace(mscclAmdSquareSum_t plan) {
-  return plan && plan->magic == kSumMagic ? plan->blocks * sizeof(double) : 0;
+  return plan && plan->magic == kSumMagic ? sumScratch(plan) : 0;
 }
 
 ncclResult_t mscclAmdSquareSum(mscclAmdSquareSum_t plan, double* out, void* workspace, size_t workspaceBytes,
@@ -130,8 +132,8 @@ ncclResult_t mscclAmdSquareSum(mscclAmdSquareSum_t plan, double* out, void* work
   const char* name = "mscclAmdSquareSum";
   if (!plan || plan->magic != kSumMagic) REFUSE("%s : invalid plan", name);
   if (!out || !aligned(out, 8)) REFUSE("%s : out is NULL or not aligned", name);
-  if (!workspace || !aligned(workspace, 8) || workspaceBytes < plan->blocks * sizeof(double))
-    REFUSE("%s : needs %zu bytes of workspace at an 8-byte boundary", name, plan->blocks * sizeof(double));
+  if (sumScratch(plan) && (!workspace || !aligned(workspace, 8) || workspaceBytes < sumScratch(plan)))
+    REFUSE("%s : needs %zu bytes of workspace at an 8-byte boundary", name, sumScratch(plan));
   if (launchSquareSum(plan->tab, plan->type, out, (double*)workspace, plan->blocks, stream)) {
     WARN("%s : launch failed", name);
     return ncclUnhandledCudaError;
@@ -192,9 +194,11 @@ ncclResult_t mscclAmdAdamWCreate(mscclAmdAdamW_t* plan, const mscclAmdAdamWTenso
     }
     std::vector<uint64_t> image;
     uint32_t chunks;
-    if (!makeTable(&image, rows.data(), n, &chunks)) REFUSE("%s : too many elements", name);
+    if (!makeTable(&image, rows.data(), n, kAdamChunk, &chunks)) REFUSE("%s : too many elements", name);
+    // the control block (zeros) and the table
+    image.insert(image.begin(), sizeof(AdamControl) / 8, 0);
     char* table = (char*)device + sizeof(AdamControl);
-    if (launchTableWrite(table, image.data(), image.size() * 8, stream)) {
+    if (launchTableWrite(device, image.data(), image.size() * 8, stream)) {
       WARN("%s : launch failed", name);
       return ncclUnhandledCudaError;
     }
@@ -299,7 +303,8 @@ static ncclResult_t checkRouter(const char* name, const mscclAmdRouter_t* r, boo
 
 size_t mscclAmdBalanceWorkspace(size_t tokens, size_t experts) {
   if (tokens > (size_t)1 << 30 || experts < 1 || experts > (size_t)kMaxExperts) return 0;
-  return (size_t)balanceBlocks((int64_t)tokens, (int)experts) * (2 * experts + 1) * 4;
+  const size_t blocks = (size_t)balanceBlocks((int64_t)tokens, (int)experts);
+  return blocks == 1 ? 0 : blocks * (2 * experts + 1) * 4;
 }
 
 ncclResult_t mscclAmdBalanceStats(const mscclAmdRouter_t* router, int64_t* counts, float* probs, void* workspace,
@@ -309,7 +314,7 @@ ncclResult_t mscclAmdBalanceStats(const mscclAmdRouter_t* router, int64_t* count
   NCCLCHECK(checkRouter(name, router, true, &a));
   if (!counts || !probs || !aligned(counts, 8) || !aligned(probs, 4)) REFUSE("%s : counts or probs is NULL or not aligned", name);
   const size_t need = mscclAmdBalanceWorkspace(router->tokens, router->experts);
-  if (!workspace || !aligned(workspace, 4) || workspaceBytes < need)
+  if (need && (!workspace || !aligned(workspace, 4) || workspaceBytes < need))
     REFUSE("%s : needs %zu bytes of workspace at a 4-byte boundary", name, need);
   const int blocks = balanceBlocks(a.tokens, a.experts);
   a.counts = counts;

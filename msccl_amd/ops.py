@@ -69,24 +69,24 @@ def _lib():
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The handle of the device's current stream (without a Stream object: it sits on every call's path)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class _on:
-    """Makes `device` the current one if it is not (the launches go to the current device)."""
-    __slots__ = ("guard",)
-
-    def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
+class _Here:
     def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
+        return self
 
     def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
         return False
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """Makes `device` the current one if it is not (the launches go to the current device)."""
+    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _flat(t, what: str, dtypes, device=None, numel: Optional[int] = None) -> None:
@@ -173,11 +173,11 @@ class SquareSum(_Plan):
             _flat(out, "out", (torch.float64,), self.device, 1)
         with _on(self.device):
             # scratch of this call's own: calls on several streams, or in several graphs, do not meet in it
-            scratch = torch.empty(self._scratch // 8 + 1, dtype=torch.float64, device=self.device)
+            scratch = torch.empty(self._scratch, dtype=torch.uint8, device=self.device) if self._scratch else None
             if out is None:
                 out = torch.empty(1, dtype=torch.float64, device=self.device)
-            rc = _lib().mscclAmdSquareSum(self.handle, out.data_ptr(), scratch.data_ptr(), self._scratch,
-                                          _stream(self.device))
+            rc = _lib().mscclAmdSquareSum(self.handle, out.data_ptr(), scratch.data_ptr() if self._scratch else None,
+                                          self._scratch, _stream(self.device))
         if rc:
             raise NcclError(rc, "mscclAmdSquareSum")
         return out
@@ -357,6 +357,8 @@ def _router(logits, index, top_k, valid, score) -> _Router:
         raise ValueError("logits: a row's elements must be neighbours, and rows must not overlap")
     r = _Router()
     r.logits, r.type, r.tokens, r.experts = logits.data_ptr(), _TYPES[logits.dtype], t, e
+    if e > 1024:
+        raise ValueError("%d experts: at most 1024" % e)
     r.logit_stride = logits.stride(0) if t > 1 else e
     if index is not None:
         if not isinstance(index, torch.Tensor) or index.dtype not in _INDEX or index.dim() != 2 or index.shape[0] != t:
@@ -391,13 +393,11 @@ def balance_stats(logits: torch.Tensor, index: torch.Tensor, valid: Optional[tor
     L = _lib()
     with _on(dev):
         size = L.mscclAmdBalanceWorkspace(r.tokens, r.experts)
-        if not size:
-            raise ValueError("%d tokens over %d experts: at most 2^30 tokens, 1 to 1024 experts" % (r.tokens, r.experts))
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         counts = torch.empty(r.experts + 1, dtype=torch.int64, device=dev)
         probs = torch.empty(r.experts, dtype=torch.float32, device=dev)
-        rc = L.mscclAmdBalanceStats(ctypes.byref(r), counts.data_ptr(), probs.data_ptr(), scratch.data_ptr(), size,
-                                    _stream(dev))
+        rc = L.mscclAmdBalanceStats(ctypes.byref(r), counts.data_ptr(), probs.data_ptr(),
+                                    scratch.data_ptr() if size else None, size, _stream(dev))
     if rc:
         raise NcclError(rc, "mscclAmdBalanceStats")
     return counts, probs

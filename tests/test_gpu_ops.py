@@ -454,13 +454,17 @@ def scores64(x, score):
 
 
 def rows_error(x, score):
-    """Roundings of a probability, in u: the exponent's (its argument's size: the subtraction rounds by u of
-    it), 4 of the exponential, the sum's 15, the reciprocal's and the product's 2 each, and the sum's terms' own."""
-    if score == "sigmoid":
-        return 60.0
+    """Roundings of a probability, in u.  softmax, of a logit d below its row's largest: 1 d of the
+    subtraction and 1.3 d of the product with log2(e) (its rounding and the constant's) in the exponential,
+    whose own are 2; the same of the sum's terms, which weigh as p does, and sum p d <= 2 + ln 1024 = 9: 23;
+    the sum's 15 additions, the reciprocal's 2 and the product's 1: 2.3 d + 43.  sigmoid: 1.3 |x| + 2 of
+    the exponential, 1 of 1 + e, the reciprocal's 2, a product: 1.3 |x| + 6, twice with the sum's terms, its
+    15 additions, the quotient and the product's 2: 2.6 |x| + 30."""
     x = x.double()
     fine = torch.where(torch.isfinite(x), x, 0.0)
-    return 2 * (fine.amax(1, keepdim=True) - fine.amin(1, keepdim=True)) + 40
+    if score == "sigmoid":
+        return 2.6 * fine.abs().amax(1, keepdim=True) + 30
+    return 2.3 * (fine.amax(1, keepdim=True) - fine.amin(1, keepdim=True)) + 43
 
 
 def router(tokens, experts, k, dtype, masked, seed=3, index=torch.int32, pad=0, scale=2.0):

@@ -104,9 +104,9 @@ def test_balance_stats_refuses(kw):
 
 
 def test_balance_stats_refuses_outputs():
-    L, r = ops._lib(), router()
-    need = L.mscclAmdBalanceWorkspace(10, 8)
-    assert need > 0
+    L, r = ops._lib(), router(tokens=50000)
+    need = L.mscclAmdBalanceWorkspace(50000, 8)
+    assert need > 0 and L.mscclAmdBalanceWorkspace(10, 8) == 0
     for args in [(None, A, A, need), (A, None, A, need), (A, A, None, need), (A, A, A, need - 1), (A + 4, A, A, need),
                  (A, A + 2, A, need), (A, A, A + 2, need)]:
         assert L.mscclAmdBalanceStats(ctypes.byref(r), *args, None) == BAD
