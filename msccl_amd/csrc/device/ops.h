@@ -11,8 +11,9 @@ namespace msccl {
 constexpr int kOpsThreads = 256;
 constexpr int kStateBlock = 256;     // elements that share a scale in 8-bit states
 // elements of one tensor that a workgroup takes at a time
-constexpr int kAdamEach = 8;         // elements a lane
-constexpr uint32_t kAdamChunk = kOpsThreads * kAdamEach;
+// (AdamW: `wide`, where a tensor beside 8-bit states is in 32 bits)
+constexpr int adamEach(int bits, bool wide) { return bits == 8 && wide ? 4 : 8; }   // elements a lane
+constexpr uint32_t adamChunk(int bits, bool wide) { return kOpsThreads * adamEach(bits, wide); }
 constexpr int kSumVecs = 4;          // 16-byte vectors a lane
 constexpr uint32_t sumChunk(size_t elemSize) { return kOpsThreads * (16 / elemSize) * kSumVecs; }
 

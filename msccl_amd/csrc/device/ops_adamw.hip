@@ -4,10 +4,11 @@
 // p = p (1 - lr decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps).  Nothing is used twice, so
 // the step is bound by HBM: 28 bytes an element (32-bit weights, or 16-bit ones with a 32-bit copy, and
 // 32-bit moments), 16 or 10 with the moments in a byte each.  One launch takes every tensor: a workgroup
-// takes 2048-element chunks, and finds the chunk's tensor in the table with one ballot a round.  A lane
-// takes twice 4 neighbours, so that a wave's 32-bit loads and stores are whole lines one after the
-// other; with states in 8 bits it takes 8 neighbours at once, so that a run of 256 elements that share
-// a scale is half a wave and its largest magnitude five lane exchanges away.
+// takes a chunk, and finds the chunk's tensor in the table with one ballot a round.  A lane takes 4
+// neighbours at a time, so that a wave's 32-bit loads and stores are whole lines one after the other:
+// twice with 32-bit states (67M weights: 318 us, once 341), once with 8-bit states beside 32-bit tensors
+// (134M: 350 us, twice 369).  Where 8-bit states stand beside 16-bit tensors alone it takes 8 neighbours,
+// 16 bytes of those (46M: 80 us, twice 4 82, once 4 89).  256 elements that share a scale are then one or half a wave's.
 #include "ops.h"
 
 namespace msccl {
@@ -188,8 +189,9 @@ struct AdamChunk {
 // stand together without branches); else `left` elements are.
 template <class P, class G, bool MASTER, int BITS, bool FULL>
 __device__ __forceinline__ void adamwChunk(const AdamStepArgs& a, const AdamChunk& t, uint64_t from, int left) {
-  constexpr int N = BITS == 8 ? 8 : 4;
-  constexpr int J = kAdamEach / N;
+  constexpr bool wide = MASTER || sizeof(P) == 4 || sizeof(G) == 4;
+  constexpr int N = BITS == 8 && !wide ? 8 : 4;
+  constexpr int J = adamEach(BITS, wide) / N;
   constexpr int runLanes = kStateBlock / N;
   typedef typename VecOf<float, N>::F F;
   F g[J], p[J], m[J], v[J];
@@ -283,16 +285,17 @@ __global__ void __launch_bounds__(kOpsThreads) adamwKernel(AdamStepArgs a) {
     ctl.rate = scalarLoad(&a.ctl->rate);
   }
   if (ctl.skip) return;
+  constexpr uint32_t chunk = adamChunk(BITS, MASTER || sizeof(P) == 4 || sizeof(G) == 4);
   for (uint32_t c = blockIdx.x; c < a.tab.chunks; c += gridDim.x) {
     const uint32_t ti = findTensor(a.tab.starts, a.tab.n, c);
     const AdamTensor* t = a.tab.rows + ti;
-    const uint64_t from = (uint64_t)(c - scalarLoad(a.tab.starts + ti)) * kAdamChunk;
+    const uint64_t from = (uint64_t)(c - scalarLoad(a.tab.starts + ti)) * chunk;
     const uint64_t left = scalarLoad(&t->count) - from;
     const double lrScale = scalarLoad(&t->lrScale);
     const AdamChunk k = {scalarLoad(&t->param), scalarLoad(&t->grad), scalarLoad(&t->master), (char*)scalarLoad(&t->m),
                          (char*)scalarLoad(&t->v), scalarLoad(&t->mScale), scalarLoad(&t->vScale), ctl.coef, ctl.invRoot,
                          (float)(1.0 - ctl.lr * lrScale * scalarLoad(&t->decay)), (float)(ctl.rate * lrScale)};
-    if (left >= kAdamChunk) adamwChunk<P, G, MASTER, BITS, true>(a, k, from, 0);
+    if (left >= chunk) adamwChunk<P, G, MASTER, BITS, true>(a, k, from, 0);
     else adamwChunk<P, G, MASTER, BITS, false>(a, k, from, (int)left);
   }
 }

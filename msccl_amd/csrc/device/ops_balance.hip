@@ -8,16 +8,19 @@
 // the sums over a row are lane exchanges.  A lane's columns are the same in every row it takes: the
 // sums over rows stay in its registers too, then one exchange through LDS and one partial sum a
 // workgroup, which a second launch adds in a fixed order in 64 bits.  Counts are integers: their
-// atomics (in LDS) give the same result in any order.  The statistics' workgroups have 1024 threads:
-// two of them fill a CU, and there are few partial sums to add.
+// atomics (in LDS) give the same result in any order.  The statistics' workgroups are large and
+// few, one a CU, so that there are few partial sums to add; the row after the one that is worked on
+// is always on its way.
 #include "ops.h"
 
 namespace msccl {
 
-// e^x for x <= 0 as 2^(x log2 e): the product's rounding and the constant's are 1.3 units of 2^-24 times
-// |x| in the result, and the hardware's 2^t is within a unit of the last place.  What is far below the
-// row's maximum, where |x| is large, weighs as little; -inf gives 0.
-__device__ __forceinline__ float expNeg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+// e^x as 2^(x log2 e); the hardware's 2^t is within a unit of the last place.
+constexpr float kLog2e = 1.44269502f;
+__device__ __forceinline__ float exp2Of(float t) { return __builtin_amdgcn_exp2f(t); }
+
+// max(a, b), or b where a is not a number; one instruction (the library's makes its operands quiet first)
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
 
 // The row's unnormalised scores in place of its logits: e^(x - max) or sigmoid(x) (0 outside the row).
 // Returns the lane's part of their sum.  SLOPE: also 1 - sigmoid(x), which 1 - s would round away near 1.
@@ -30,7 +33,7 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         // e = e^-|x|: 1 / (1 + e), or e / (1 + e) left of zero (the reciprocal of 1 to 2: within one unit)
-        const float e = expNeg(-fabsf(x[j][i]));
+        const float e = exp2Of(-fabsf(x[j][i]) * kLog2e);
         const float r = __builtin_amdgcn_rcpf(1.f + e), er = e * r;
         const bool right = x[j][i] >= 0.f;
         if constexpr (SLOPE) slope[j][i] = right ? er : r;
@@ -42,17 +45,28 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
 #pragma unroll
     for (int j = 0; j < VPL; j++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) top = fmaxf(top, x[j][i]);
+      for (int i = 0; i < 8; i++) top = larger(x[j][i], top);
     top = maxOver<LPR>(top);
-    // a row of -inf alone has no scores; its sum stays 0
-    const float from = top == -__builtin_inff() ? 0.f : top;
+    if (__builtin_expect(__ballot(!(fabsf(top) < 0x1p126f)) != 0, 0)) {
+      // Masked with the lowest value, infinite or nothing there: the difference itself.  A row of -inf alone
+      // has no scores; its sum stays 0.
+      const float from = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+      for (int j = 0; j < VPL; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[j][i] = exp2Of((x[j][i] - from) * kLog2e);
+    } else {
+      // One FMA: the rounding of top log2(e) is the same factor on every score of the row.
+      const float from = -top * kLog2e;
+#pragma unroll
+      for (int j = 0; j < VPL; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[j][i] = exp2Of(fmaf(x[j][i], kLog2e, from));
+    }
 #pragma unroll
     for (int j = 0; j < VPL; j++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        x[j][i] = expNeg(x[j][i] - from);
-        sum += x[j][i];
-      }
+      for (int i = 0; i < 8; i++) sum += x[j][i];
   }
   return sum;
 }
@@ -80,19 +94,22 @@ struct Columns {
   __device__ __forceinline__ bool has(int i) const { return i >= skip && i < end; }
 };
 
-// The lane's eight of a row; `none` in the place of columns that are not its own.
+// The lane's eight of a row as they stand, and as 32-bit values with `none` in the place of columns that
+// are not its own.
 template <class T, int LPR>
-__device__ __forceinline__ f32x8 loadRow(const T* row, const Columns& c, float none) {
-  f32x8 x;
+__device__ __forceinline__ typename VecOf<T, 8>::V loadRow(const T* row, const Columns& c) {
+  typename VecOf<T, 8>::V x;
   if (LPR == 1 && c.end < 8) {
-    T y[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[i] = inGlobal(row)[i < c.end ? i : c.end - 1];
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)y[i];
+    for (int i = 0; i < 8; i++) x[i] = inGlobal(row)[i < c.end ? i : c.end - 1];
   } else {
-    x = __builtin_convertvector(loadVec<8>(row + c.base), f32x8);
+    x = loadVec<8>(row + c.base);
   }
+  return x;
+}
+template <class V>
+__device__ __forceinline__ f32x8 ownColumns(const V& raw, const Columns& c, float none) {
+  f32x8 x = __builtin_convertvector(raw, f32x8);
   if (!c.whole) {
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = c.has(i) ? x[i] : none;
@@ -109,40 +126,67 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
   constexpr int waves = kStatsThreads / 64;
   constexpr int copies = width <= 128 ? waves : 1;   // few experts: every wave counts by itself
   __shared__ uint32_t hist[copies][width];
-  __shared__ uint32_t valid;
+  __shared__ uint32_t tokens;
   __shared__ float sums[waves / 2][width];
   const int wave = threadIdx.x / 64;
   const int64_t begin = blockIdx.x * rowsEach;
   const int64_t first = begin < a.tokens ? begin : a.tokens;   // (the last workgroups may have none)
   const int64_t end = a.tokens - first < rowsEach ? a.tokens : first + rowsEach;
 
-  for (int i = threadIdx.x; i < copies * width; i += kStatsThreads) (&hist[0][0])[i] = 0;
-  if (threadIdx.x == 0) valid = 0;
-  __syncthreads();
-  const uint32_t slots = (uint32_t)(end - first) * (uint32_t)a.topK;
-  for (uint32_t s = threadIdx.x; s < slots; s += kStatsThreads) {
-    const uint32_t r = s / (uint32_t)a.topK;
-    const int64_t row = first + r;
-    const int64_t at = row * a.indexStride + (s - r * (uint32_t)a.topK);
-    const bool here = !a.valid || inGlobal(a.valid)[row];
-    const int64_t e = IDX64 ? inGlobal((const int64_t*)a.index)[at] : (int64_t)inGlobal((const int32_t*)a.index)[at];
-    if (here && (uint64_t)e < (uint64_t)a.experts) atomicAdd(&hist[copies == 1 ? 0 : wave][e], 1u);
+  const int lane = threadIdx.x % LPR, own = threadIdx.x / LPR;
+  const Columns c0(a.experts, width, lane * 8), c1(a.experts, width, (LPR + lane) * 8);
+  const int rows = (int)(end - first);
+  const int64_t ahead = (int64_t)rowsPer * a.logitStride;
+  const T* at = (const T*)a.logits + (first + own) * a.logitStride;
+  const uint8_t* ok = a.valid ? a.valid + first : nullptr;
+  // a row is on its way while the one before it, and at first the choices, are worked on
+  typename VecOf<T, 8>::V raw[VPL];
+  bool valid = true;
+  if (own < rows) {
+    raw[0] = loadRow<T, LPR>(at, c0);
+    if constexpr (VPL == 2) raw[1] = loadRow<T, LPR>(at, c1);
+    if (ok) valid = inGlobal(ok)[own];
   }
 
-  const int lane = threadIdx.x % LPR;
-  const Columns c0(a.experts, width, lane * 8), c1(a.experts, width, (LPR + lane) * 8);
-  const float none = -__builtin_inff();
+  for (int i = threadIdx.x; i < copies * width; i += kStatsThreads) (&hist[0][0])[i] = 0;
+  if (threadIdx.x == 0) tokens = 0;
+  __syncthreads();
+  const uint32_t slots = (uint32_t)rows * (uint32_t)a.topK;
+  const bool packed = !ok && a.indexStride == a.topK;   // slot s of the rows is element s
+  for (uint32_t s0 = threadIdx.x; s0 < slots; s0 += 4 * kStatsThreads) {
+    int64_t e[4];   // four on their way at once
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const uint32_t s = s0 + k * kStatsThreads;
+      e[k] = -1;
+      if (s >= slots) continue;
+      const uint32_t r = packed ? 0 : s / (uint32_t)a.topK;
+      const int64_t i = (first + r) * a.indexStride + (s - r * (uint32_t)a.topK);
+      if (!ok || inGlobal(ok)[r])
+        e[k] = IDX64 ? inGlobal((const int64_t*)a.index)[i] : (int64_t)inGlobal((const int32_t*)a.index)[i];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+      if ((uint64_t)e[k] < (uint64_t)a.experts) atomicAdd(&hist[copies == 1 ? 0 : wave][e[k]], 1u);
+  }
+
   f32x8 acc[VPL];
 #pragma unroll
   for (int j = 0; j < VPL; j++) acc[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};
   uint32_t here = 0;
-  for (int64_t row = first + threadIdx.x / LPR; row < end; row += rowsPer) {
-    if (a.valid && !inGlobal(a.valid)[row]) continue;
-    here++;
-    const T* at = (const T*)a.logits + row * a.logitStride;
+  for (int r = own; r < rows; r += rowsPer) {
     f32x8 x[VPL];
-    x[0] = loadRow<T, LPR>(at, c0, none);
-    if constexpr (VPL == 2) x[1] = loadRow<T, LPR>(at, c1, none);
+    x[0] = ownColumns(raw[0], c0, -__builtin_inff());
+    if constexpr (VPL == 2) x[1] = ownColumns(raw[1], c1, -__builtin_inff());
+    const bool now = valid;
+    if (r + rowsPer < rows) {
+      at += ahead;
+      raw[0] = loadRow<T, LPR>(at, c0);
+      if constexpr (VPL == 2) raw[1] = loadRow<T, LPR>(at, c1);
+      if (ok) valid = inGlobal(ok)[r + rowsPer];
+    }
+    if (!now) continue;   // (whatever the row holds)
+    here++;
     const float z = sumOver<LPR>(scores<LPR, VPL, SIG, false>(x, nullptr));
     const float inv = inverse<SIG>(z);
 #pragma unroll
@@ -150,7 +194,7 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
 #pragma unroll
       for (int i = 0; i < 8; i++) acc[j][i] = fmaf(x[j][i], inv, acc[j][i]);
   }
-  if (here && lane == 0) atomicAdd(&valid, here);
+  if (here && lane == 0) atomicAdd(&tokens, here);
   // over the wave's rows, then over the waves: the upper half's on top of the lower half's
 #pragma unroll
   for (int half = 1; half >= 0; half--) {
@@ -188,45 +232,54 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
     }
   }
   if (threadIdx.x == 0) {
-    if (only) a.counts[a.experts] = valid;
-    else a.countPart[(size_t)blockIdx.x * (a.experts + 1) + a.experts] = valid;
+    if (only) a.counts[a.experts] = tokens;
+    else a.countPart[(size_t)blockIdx.x * (a.experts + 1) + a.experts] = tokens;
   }
 }
 
-// The partial sums of at most kStatsBlocks workgroups: 32 columns a workgroup, 32 threads down each, all
+// The partial sums of at most kStatsBlocks workgroups: 16 columns a workgroup, 64 threads down each, all
 // loads of a thread under way at once.
-constexpr int kStatsBlocks = 512;
+constexpr int kStatsBlocks = 256;
 
 __global__ void __launch_bounds__(1024) balanceFinishKernel(BalanceArgs a, int blocks) {
-  __shared__ double ps[32][32];
-  __shared__ int64_t cs[32][32];
-  const int col = threadIdx.x % 32, slice = threadIdx.x / 32;
-  const int e = blockIdx.x * 32 + col;
-  float p[kStatsBlocks / 32];
-  uint32_t c[kStatsBlocks / 32];
+  constexpr int each = kStatsBlocks / 64;
+  __shared__ double ps[16][16];
+  __shared__ int64_t cs[16][16];
+  const int col = threadIdx.x % 16, slice = threadIdx.x / 16;
+  const int e = blockIdx.x * 16 + col;
+  float p[each];
+  uint32_t c[each];
 #pragma unroll
-  for (int k = 0; k < kStatsBlocks / 32; k++) {
-    const int b = k * 32 + slice;
+  for (int k = 0; k < each; k++) {
+    const int b = k * 64 + slice;
     p[k] = b < blocks && e < a.experts ? a.probPart[(size_t)b * a.experts + e] : 0.f;
     c[k] = b < blocks && e <= a.experts ? a.countPart[(size_t)b * (a.experts + 1) + e] : 0;
   }
-  double ps0 = 0.0;
-  int64_t cs0 = 0;
+  double p0 = 0.0;
+  int64_t c0 = 0;
 #pragma unroll
-  for (int k = 0; k < kStatsBlocks / 32; k++) {
-    ps0 += (double)p[k];
-    cs0 += (int64_t)c[k];
+  for (int k = 0; k < each; k++) {
+    p0 += (double)p[k];
+    c0 += (int64_t)c[k];
   }
-  ps[slice][col] = ps0;
-  cs[slice][col] = cs0;
+#pragma unroll
+  for (int d = 16; d <= 32; d *= 2) {
+    p0 += __shfl_xor(p0, d);
+    c0 += __shfl_xor((long long)c0, d);
+  }
+  if ((threadIdx.x & 63) < 16) {
+    ps[threadIdx.x / 64][col] = p0;
+    cs[threadIdx.x / 64][col] = c0;
+  }
   __syncthreads();
-  if (threadIdx.x < 32 && e <= a.experts) {
-    for (int k = 1; k < 32; k++) {
-      ps0 += ps[k][col];
-      cs0 += cs[k][col];
+  if (threadIdx.x < 16 && e <= a.experts) {
+#pragma unroll
+    for (int k = 1; k < 16; k++) {
+      p0 += ps[k][col];
+      c0 += cs[k][col];
     }
-    if (e < a.experts) a.probs[e] = (float)ps0;
-    a.counts[e] = cs0;
+    if (e < a.experts) a.probs[e] = (float)p0;
+    a.counts[e] = c0;
   }
 }
 
@@ -248,6 +301,17 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
   const int lane = threadIdx.x % LPR;
   constexpr int width = LPR * VPL * 8;
   const Columns c0(a.experts, width, lane * 8), c1(a.experts, width, (LPR + lane) * 8);
+  const int64_t ahead = (int64_t)gridDim.x * rowsPer, first = (int64_t)blockIdx.x * rowsPer + threadIdx.x / LPR;
+  const T* in = (const T*)a.logits + first * a.logitStride;
+  T* out = (T*)a.grad + first * a.gradStride;
+  // as in the statistics, a row is on its way while the one before it is worked on
+  typename VecOf<T, 8>::V raw[VPL];
+  bool next = true;
+  if (first < a.tokens) {
+    raw[0] = loadRow<T, LPR>(in, c0);
+    if constexpr (VPL == 2) raw[1] = loadRow<T, LPR>(in, c1);
+    if (a.valid) next = inGlobal(a.valid)[first];
+  }
   const double n = (double)a.countsIn[a.experts];
   // Every weight less c E / (k N^2) times the mean count of a routing that drops nothing, k N / E: p sums
   // to 1, so the gradient is the same, and with weights that are nearly equal nothing cancels in 32 bits.
@@ -260,33 +324,34 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
 #pragma unroll
     for (int i = 0; i < 8; i++) w[j][i] = c.has(i) ? (float)(((double)a.countsIn[c.base + i] - mean) * up) : 0.f;
   }
-  for (int64_t row = (int64_t)blockIdx.x * rowsPer + threadIdx.x / LPR; row < a.tokens;
-       row += (int64_t)gridDim.x * rowsPer) {
-    const bool valid = !a.valid || inGlobal(a.valid)[row];
-    if (ACC && !valid) continue;
-    const T* in = (const T*)a.logits + row * a.logitStride;
-    T* out = (T*)a.grad + row * a.gradStride;
+  for (int64_t row = first; row < a.tokens; row += ahead, out += ahead * a.gradStride) {
     f32x8 x[VPL], slope[VPL];
+    x[0] = ownColumns(raw[0], c0, -__builtin_inff());
+    if constexpr (VPL == 2) x[1] = ownColumns(raw[1], c1, -__builtin_inff());
+    const bool valid = next;
+    if (row + ahead < a.tokens) {
+      in += ahead * a.logitStride;
+      raw[0] = loadRow<T, LPR>(in, c0);
+      if constexpr (VPL == 2) raw[1] = loadRow<T, LPR>(in, c1);
+      if (a.valid) next = inGlobal(a.valid)[row + ahead];
+    }
+    if (ACC && !valid) continue;
     if (valid) {
-      x[0] = loadRow<T, LPR>(in, c0, -__builtin_inff());
-      if constexpr (VPL == 2) x[1] = loadRow<T, LPR>(in, c1, -__builtin_inff());
       const float mine = scores<LPR, VPL, SIG, SIG>(x, slope);
       float dot = 0.f;
 #pragma unroll
       for (int j = 0; j < VPL; j++)
 #pragma unroll
         for (int i = 0; i < 8; i++) dot = fmaf(x[j][i], w[j][i], dot);
-      const float z = sumOver<LPR>(mine);
-      dot = sumOver<LPR>(dot);
-      const float inv = inverse<SIG>(z);
-      dot *= inv;
+      const float inv = inverse<SIG>(sumOver<LPR>(mine));
+      // p (w - sum of w p) = s (w / z - (sum of w s) / z^2)
+      dot = sumOver<LPR>(dot) * inv * inv;
 #pragma unroll
       for (int j = 0; j < VPL; j++)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-          float d = x[j][i] * inv * (w[j][i] - dot);
-          if constexpr (SIG) d *= slope[j][i];
-          x[j][i] = d;
+          x[j][i] *= fmaf(w[j][i], inv, -dot);
+          if constexpr (SIG) x[j][i] *= slope[j][i];
         }
     } else {
 #pragma unroll
@@ -295,7 +360,7 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
 #pragma unroll
     for (int j = 0; j < VPL; j++) {
       const Columns& c = j ? c1 : c0;
-      if constexpr (ACC) x[j] += loadRow<T, LPR>(out, c, 0.f);
+      if constexpr (ACC) x[j] += ownColumns(loadRow<T, LPR>(out, c), c, 0.f);
       if (c.whole || (c.skip == 0 && c.end == 8)) {
         storeN<8>(out + c.base, x[j], 8);
       } else {
@@ -307,7 +372,7 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
   }
 }
 
-// ---- variants: the fewest lanes that hold a row, 8 logits each (two times 8 past 512 experts) --------
+// ---- variants: the fewest lanes that hold a row, 8 logits each (64 lanes 16 past 512 experts) ----------
 
 static int lanesPerRow(int experts) {
   int l = 1;
@@ -362,7 +427,7 @@ struct Backward {
     static int run(const BalanceArgs* a, bool sigmoid, bool accumulate, hipStream_t s) {
       constexpr int64_t rowsPer = kOpsThreads / LPR;
       const int64_t passes = (a->tokens + rowsPer - 1) / rowsPer;
-      const dim3 g((uint32_t)(passes < 2048 ? passes : 2048)), b(kOpsThreads);
+      const dim3 g((uint32_t)(passes < 1024 ? passes : 1024)), b(kOpsThreads);
       if (sigmoid) {
         if (accumulate) hipLaunchKernelGGL((balanceBackwardKernel<T, LPR, VPL, true, true>), g, b, 0, s, *a);
         else hipLaunchKernelGGL((balanceBackwardKernel<T, LPR, VPL, true, false>), g, b, 0, s, *a);
@@ -384,7 +449,7 @@ int launchBalanceStats(const BalanceArgs& a, int type, bool index64, bool sigmoi
     case 9: r = pick<Stats<__bf16>::template Of>(a.experts, &a, index64, sigmoid, blocks, s); break;
   }
   if (r != 0 || blocks == 1) return r;
-  hipLaunchKernelGGL(balanceFinishKernel, dim3((a.experts + 1 + 31) / 32), dim3(1024), 0, s, a, blocks);
+  hipLaunchKernelGGL(balanceFinishKernel, dim3((a.experts + 1 + 15) / 16), dim3(1024), 0, s, a, blocks);
   return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 

@@ -194,7 +194,7 @@ ncclResult_t mscclAmdAdamWCreate(mscclAmdAdamW_t* plan, const mscclAmdAdamWTenso
     }
     std::vector<uint64_t> image;
     uint32_t chunks;
-    if (!makeTable(&image, rows.data(), n, kAdamChunk, &chunks)) REFUSE("%s : too many elements", name);
+    if (!makeTable(&image, rows.data(), n, adamChunk(stateBits, master || ps == 4 || gs == 4), &chunks)) REFUSE("%s : too many elements", name);
     // the control block (zeros) and the table
     image.insert(image.begin(), sizeof(AdamControl) / 8, 0);
     char* table = (char*)device + sizeof(AdamControl);

@@ -12,6 +12,7 @@ the capture, and must outlive the graph, as their tensors must).  Wrong argument
 TypeError here, or NcclError from the library.
 """
 import ctypes
+import struct
 from typing import Optional, Sequence, Union
 
 import torch
@@ -31,11 +32,8 @@ class _AdamWTensor(ctypes.Structure):
                 ("count", ctypes.c_size_t), ("weight_decay", ctypes.c_double), ("lr_scale", ctypes.c_double)]
 
 
-class _Router(ctypes.Structure):
-    _fields_ = [("logits", ctypes.c_void_p), ("type", ctypes.c_int), ("tokens", ctypes.c_size_t),
-                ("experts", ctypes.c_size_t), ("logit_stride", ctypes.c_size_t), ("index", ctypes.c_void_p),
-                ("index_type", ctypes.c_int), ("top_k", ctypes.c_size_t), ("index_stride", ctypes.c_size_t),
-                ("valid", ctypes.c_void_p), ("score", ctypes.c_int)]
+# mscclAmdRouter_t: logits, type, tokens, experts, logitStride, index, indexType, topK, indexStride, valid, score
+_ROUTER = struct.Struct("@PiNNNPiNNPi")
 
 
 _L = None
@@ -61,9 +59,9 @@ def _lib():
         L.mscclAmdAdamWDestroy.argtypes = [vp]
         L.mscclAmdBalanceWorkspace.argtypes = [sz, sz]
         L.mscclAmdBalanceWorkspace.restype = sz
-        L.mscclAmdBalanceStats.argtypes = [ctypes.POINTER(_Router), vp, vp, vp, sz, vp]
+        L.mscclAmdBalanceStats.argtypes = [ctypes.c_char_p, vp, vp, vp, sz, vp]
         L.mscclAmdBalanceLoss.argtypes = [vp, vp, sz, sz, d, vp, vp]
-        L.mscclAmdBalanceBackward.argtypes = [ctypes.POINTER(_Router), vp, d, vp, vp, sz, i, vp]
+        L.mscclAmdBalanceBackward.argtypes = [ctypes.c_char_p, vp, d, vp, vp, sz, i, vp]
         _L = L
     return _L
 
@@ -73,20 +71,9 @@ def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def _on(device):
-    """Makes `device` the current one if it is not (the launches go to the current device)."""
-    return _HERE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+def _elsewhere(device) -> bool:
+    """Whether another device is the current one (the launches go to the current device)."""
+    return torch._C._cuda_getDevice() != device.index
 
 
 def _flat(t, what: str, dtypes, device=None, numel: Optional[int] = None) -> None:
@@ -171,13 +158,16 @@ class SquareSum(_Plan):
         self._live()
         if out is not None:
             _flat(out, "out", (torch.float64,), self.device, 1)
-        with _on(self.device):
-            # scratch of this call's own: calls on several streams, or in several graphs, do not meet in it
-            scratch = torch.empty(self._scratch, dtype=torch.uint8, device=self.device) if self._scratch else None
-            if out is None:
-                out = torch.empty(1, dtype=torch.float64, device=self.device)
-            rc = _lib().mscclAmdSquareSum(self.handle, out.data_ptr(), scratch.data_ptr() if self._scratch else None,
-                                          self._scratch, _stream(self.device))
+        dev = self.device
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self(out)
+        # scratch of this call's own: calls on several streams, or in several graphs, do not meet in it
+        scratch = torch.empty(self._scratch, dtype=torch.uint8, device=dev) if self._scratch else None
+        if out is None:
+            out = torch.empty(1, dtype=torch.float64, device=dev)
+        rc = _lib().mscclAmdSquareSum(self.handle, out.data_ptr(), scratch.data_ptr() if self._scratch else None,
+                                      self._scratch, _stream(dev))
         if rc:
             raise NcclError(rc, "mscclAmdSquareSum")
         return out
@@ -273,7 +263,7 @@ class AdamW(_Plan):
         for i, g in enumerate(grads):
             _flat(g, "grads[%d]" % i, (self._grad_type,), self.device, params[i].numel())
         ptrs = (ctypes.c_void_p * len(grads))(*[g.data_ptr() for g in grads])
-        with _on(self.device):
+        with torch.cuda.device(self.device):
             _check(_lib().mscclAmdAdamWSetGrads(self.handle, ptrs, len(grads), _stream(self.device)),
                    "mscclAmdAdamWSetGrads")
         self.tensors[1] = list(grads)
@@ -295,9 +285,13 @@ class AdamW(_Plan):
             total = grad_square_sum.data_ptr()
         if max_norm is not None and not max_norm > 0:
             raise ValueError("max_norm must be above zero")
-        with _on(self.device):
-            rc = _lib().mscclAmdAdamWStep(self.handle, lr, at, betas[0], betas[1], eps, grad_scale, total,
-                                          max_norm or 0.0, _stream(self.device))
+        launch, args = _lib().mscclAmdAdamWStep, (self.handle, lr, at, betas[0], betas[1], eps, grad_scale, total,
+                                                  max_norm or 0.0, _stream(self.device))
+        if _elsewhere(self.device):
+            with torch.cuda.device(self.device):
+                rc = launch(*args)
+        else:
+            rc = launch(*args)
         if rc:
             raise NcclError(rc, "mscclAmdAdamWStep")
 
@@ -347,39 +341,40 @@ def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: S
 
 # ---- balance loss of a router's experts ----------------------------------------------------------
 
-def _router(logits, index, top_k, valid, score) -> _Router:
-    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda":
+def _rows(t: torch.Tensor, what: str, rows: int, cols: int) -> int:
+    """The stride from row to row of a matrix whose rows are whole and apart."""
+    down, along = t.stride()
+    if (cols > 1 and along != 1) or (rows > 1 and down < cols):
+        raise ValueError("%s: a row's elements must be neighbours, and rows must not overlap" % what)
+    return down if rows > 1 else cols
+
+
+def _router(logits, index, top_k, valid, score) -> bytes:
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
         raise ValueError("logits must be a tensor on a GPU")
-    if logits.dim() != 2 or logits.dtype not in _TYPES:
+    code = _TYPES.get(logits.dtype)
+    if code is None or logits.dim() != 2:
         raise TypeError("logits must be [tokens, experts] of float32, float16 or bfloat16")
     t, e = logits.shape
-    if (e > 1 and logits.stride(1) != 1) or (t > 1 and logits.stride(0) < e):
-        raise ValueError("logits: a row's elements must be neighbours, and rows must not overlap")
-    r = _Router()
-    r.logits, r.type, r.tokens, r.experts = logits.data_ptr(), _TYPES[logits.dtype], t, e
     if e > 1024:
         raise ValueError("%d experts: at most 1024" % e)
-    r.logit_stride = logits.stride(0) if t > 1 else e
+    stride = _rows(logits, "logits", t, e)
+    at = itype = istride = ok = 0
     if index is not None:
         if not isinstance(index, torch.Tensor) or index.dtype not in _INDEX or index.dim() != 2 or index.shape[0] != t:
             raise TypeError("index must be [tokens, k] of int32 or int64")
-        top_k = index.shape[1]
         if index.device != logits.device:
             raise ValueError("index is on %s, not %s" % (index.device, logits.device))
-        if (top_k > 1 and index.stride(1) != 1) or (t > 1 and index.stride(0) < top_k):
-            raise ValueError("index: a row's elements must be neighbours, and rows must not overlap")
-        r.index, r.index_type = index.data_ptr(), _INDEX[index.dtype]
-        r.index_stride = index.stride(0) if t > 1 else top_k
-    r.top_k = top_k
+        top_k = index.shape[1]
+        at, itype, istride = index.data_ptr(), _INDEX[index.dtype], _rows(index, "index", t, top_k)
+    elif not 0 < top_k <= e:
+        raise ValueError("top_k %r of %d experts" % (top_k, e))
     if valid is not None:
-        if not isinstance(valid, torch.Tensor):
-            raise TypeError("valid must be a torch tensor")
         _flat(valid, "valid", (torch.bool, torch.uint8), logits.device, t)
-        r.valid = valid.data_ptr()
+        ok = valid.data_ptr()
     if score not in _SCORES:
         raise ValueError("score %r is not one of %s" % (score, ", ".join(_SCORES)))
-    r.score = _SCORES[score]
-    return r
+    return _ROUTER.pack(logits.data_ptr(), code, t, e, stride, at, itype, top_k, istride, ok, _SCORES[score])
 
 
 def balance_stats(logits: torch.Tensor, index: torch.Tensor, valid: Optional[torch.Tensor] = None,
@@ -388,16 +383,21 @@ def balance_stats(logits: torch.Tensor, index: torch.Tensor, valid: Optional[tor
     each expert and then the number of valid tokens; probs float32 [experts], the sums over valid tokens of
     softmax(logits), or with score="sigmoid" of sigmoid(logits) over its row's sum.  index [tokens, k]: the
     chosen experts (one outside [0, experts) is a dropped slot); valid [tokens]: None, or false for padding."""
+    if index is None:
+        raise TypeError("index must be [tokens, k] of int32 or int64")
     r = _router(logits, index, 0, valid, score)
     dev = logits.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return balance_stats(logits, index, valid, score)
+    t, e = logits.shape
     L = _lib()
-    with _on(dev):
-        size = L.mscclAmdBalanceWorkspace(r.tokens, r.experts)
-        scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-        counts = torch.empty(r.experts + 1, dtype=torch.int64, device=dev)
-        probs = torch.empty(r.experts, dtype=torch.float32, device=dev)
-        rc = L.mscclAmdBalanceStats(ctypes.byref(r), counts.data_ptr(), probs.data_ptr(),
-                                    scratch.data_ptr() if size else None, size, _stream(dev))
+    size = L.mscclAmdBalanceWorkspace(t, e)
+    scratch = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    counts = torch.empty(e + 1, dtype=torch.int64, device=dev)
+    probs = torch.empty(e, dtype=torch.float32, device=dev)
+    rc = L.mscclAmdBalanceStats(r, counts.data_ptr(), probs.data_ptr(), scratch.data_ptr() if size else None, size,
+                                _stream(dev))
     if rc:
         raise NcclError(rc, "mscclAmdBalanceStats")
     return counts, probs
@@ -421,11 +421,15 @@ def balance_all_reduce(comms: Sequence[Comm], counts: Sequence[torch.Tensor], pr
 def balance_loss(counts: torch.Tensor, probs: torch.Tensor, top_k: int, coef: float = 1.0) -> torch.Tensor:
     """coef * experts / (k N^2) * sum of counts[e] * probs[e] (N valid tokens; 0 for none), float32 of one element."""
     _flat(probs, "probs", (torch.float32,))
-    _flat(counts, "counts", (torch.int64,), probs.device, probs.numel() + 1)
-    with _on(probs.device):
-        loss = torch.empty(1, dtype=torch.float32, device=probs.device)
-        rc = _lib().mscclAmdBalanceLoss(counts.data_ptr(), probs.data_ptr(), probs.numel(), top_k, coef,
-                                        loss.data_ptr(), _stream(probs.device))
+    dev, e = probs.device, probs.numel()
+    _flat(counts, "counts", (torch.int64,), dev, e + 1)
+    if not 0 < top_k <= e:
+        raise ValueError("top_k %r of %d experts" % (top_k, e))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return balance_loss(counts, probs, top_k, coef)
+    loss = torch.empty(1, dtype=torch.float32, device=dev)
+    rc = _lib().mscclAmdBalanceLoss(counts.data_ptr(), probs.data_ptr(), e, top_k, coef, loss.data_ptr(), _stream(dev))
     if rc:
         raise NcclError(rc, "mscclAmdBalanceLoss")
     return loss
@@ -439,7 +443,8 @@ def balance_backward(logits: torch.Tensor, counts: torch.Tensor, top_k: int, coe
     of one element.  out: where to write it; accumulate: it is added to what `out` holds."""
     r = _router(logits, None, top_k, valid, score)
     dev = logits.device
-    _flat(counts, "counts", (torch.int64,), dev, r.experts + 1)
+    t, e = logits.shape
+    _flat(counts, "counts", (torch.int64,), dev, e + 1)
     up = None
     if grad_output is not None:
         _flat(grad_output, "grad_output", (torch.float32,), dev, 1)
@@ -447,16 +452,18 @@ def balance_backward(logits: torch.Tensor, counts: torch.Tensor, top_k: int, coe
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        out, stride = torch.empty((t, e), dtype=logits.dtype, device=dev), e
     else:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
             raise ValueError("out must have the shape, type and device of logits")
-        if (r.experts > 1 and out.stride(1) != 1) or (r.tokens > 1 and out.stride(0) < r.experts):
-            raise ValueError("out: a row's elements must be neighbours, and rows must not overlap")
-    stride = out.stride(0) if r.tokens > 1 else r.experts
-    with _on(dev):
-        rc = _lib().mscclAmdBalanceBackward(ctypes.byref(r), counts.data_ptr(), coef, up, out.data_ptr(), stride,
-                                            int(accumulate), _stream(dev))
+        stride = _rows(out, "out", t, e)
+    launch, args = _lib().mscclAmdBalanceBackward, (r, counts.data_ptr(), coef, up, out.data_ptr(), stride,
+                                                    int(accumulate), _stream(dev))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            rc = launch(*args)
+    else:
+        rc = launch(*args)
     if rc:
         raise NcclError(rc, "mscclAmdBalanceBackward")
     return out

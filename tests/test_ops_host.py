@@ -83,13 +83,13 @@ def test_adamw_refuses_bad_plan():
     assert L.mscclAmdAdamWDestroy(ctypes.addressof(junk)) == BAD
 
 
+FIELDS = ("logits", "type", "tokens", "experts", "logit_stride", "index", "index_type", "top_k", "index_stride", "valid", "score")
+
+
 def router(**kw):
-    r = ops._Router()
     base = dict(logits=A, type=F32, tokens=10, experts=8, logit_stride=8, index=A, index_type=I32, top_k=2,
                 index_stride=2, valid=None, score=0)
-    for k, v in (base | kw).items():
-        setattr(r, k, v)
-    return r
+    return ops._ROUTER.pack(*[(base | kw)[f] or 0 for f in FIELDS])
 
 
 BAD_ROUTERS = [dict(type=I32), dict(type=M.FLOAT64), dict(score=2), dict(score=-1), dict(experts=0), dict(experts=1025),
@@ -100,7 +100,7 @@ BAD_ROUTERS = [dict(type=I32), dict(type=M.FLOAT64), dict(score=2), dict(score=-
 @pytest.mark.parametrize("kw", BAD_ROUTERS + [dict(index=None), dict(index_type=F32), dict(index_stride=1), dict(index=A + 2),
                                               dict(index_type=I64, index=A + 4), dict(index_stride=1 << 40)])
 def test_balance_stats_refuses(kw):
-    assert ops._lib().mscclAmdBalanceStats(ctypes.byref(router(**kw)), A, A, A, 1 << 30, None) == BAD
+    assert ops._lib().mscclAmdBalanceStats(router(**kw), A, A, A, 1 << 30, None) == BAD
 
 
 def test_balance_stats_refuses_outputs():
@@ -109,7 +109,7 @@ def test_balance_stats_refuses_outputs():
     assert need > 0 and L.mscclAmdBalanceWorkspace(10, 8) == 0
     for args in [(None, A, A, need), (A, None, A, need), (A, A, None, need), (A, A, A, need - 1), (A + 4, A, A, need),
                  (A, A + 2, A, need), (A, A, A + 2, need)]:
-        assert L.mscclAmdBalanceStats(ctypes.byref(r), *args, None) == BAD
+        assert L.mscclAmdBalanceStats(r, *args, None) == BAD
     assert L.mscclAmdBalanceStats(None, A, A, A, need, None) == BAD
     assert L.mscclAmdBalanceWorkspace(10, 0) == 0 and L.mscclAmdBalanceWorkspace(10, 1025) == 0
     assert L.mscclAmdBalanceWorkspace((1 << 30) + 1, 8) == 0
@@ -125,7 +125,7 @@ def test_balance_loss_refuses(args):
 
 @pytest.mark.parametrize("kw", BAD_ROUTERS)
 def test_balance_backward_refuses(kw):
-    assert ops._lib().mscclAmdBalanceBackward(ctypes.byref(router(**kw)), A, 1.0, None, 2 * A, 8, 0, None) == BAD
+    assert ops._lib().mscclAmdBalanceBackward(router(**kw), A, 1.0, None, 2 * A, 8, 0, None) == BAD
 
 
 @pytest.mark.parametrize("args", [(None, 1.0, None, 2 * A, 8, 0), (A + 4, 1.0, None, 2 * A, 8, 0), (A, float("inf"), None, 2 * A, 8, 0),
@@ -133,7 +133,7 @@ def test_balance_backward_refuses(kw):
                                   (A, 1.0, None, 2 * A, 7, 0), (A, 1.0, None, 2 * A, 1 << 40, 0),
                                   (A, 1.0, None, A, 8, 1), (A, 1.0, None, A, 9, 0)])
 def test_balance_backward_refuses_outputs(args):
-    assert ops._lib().mscclAmdBalanceBackward(ctypes.byref(router()), *args, None) == BAD
+    assert ops._lib().mscclAmdBalanceBackward(router(), *args, None) == BAD
 
 
 def test_python_refuses_host_tensors():
@@ -171,3 +171,16 @@ def test_states_and_their_values():
     scale = torch.tensor([0.5, 3.0])
     assert ops.dequantize_state(code, scale).tolist() == [1.0] * 256 + [6.0] * 44
     assert ops.dequantize_state(code, scale, second=True).tolist() == [1.0] * 256 + [36.0] * 44
+
+
+def test_router_struct_is_the_headers():
+    """The packed router against the C compiler's layout of mscclAmdRouter_t."""
+    class Router(ctypes.Structure):
+        _fields_ = [("logits", ctypes.c_void_p), ("type", ctypes.c_int), ("tokens", ctypes.c_size_t),
+                    ("experts", ctypes.c_size_t), ("logit_stride", ctypes.c_size_t), ("index", ctypes.c_void_p),
+                    ("index_type", ctypes.c_int), ("top_k", ctypes.c_size_t), ("index_stride", ctypes.c_size_t),
+                    ("valid", ctypes.c_void_p), ("score", ctypes.c_int)]
+    values = list(range(101, 112))
+    raw = ops._ROUTER.pack(*values)
+    r = Router.from_buffer_copy(raw.ljust(ctypes.sizeof(Router), b"\0"))
+    assert [getattr(r, f) for f in FIELDS] == values
