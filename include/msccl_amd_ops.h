@@ -77,7 +77,8 @@ size_t mscclAmdAdamWBytes(size_t n);
 
 /* A plan over n tensors (host array, read now; a tensor may be empty).  step: one int64 on the device,
  * the steps taken so far (0 at first), advanced by every step: it and the moments are the optimizer's
- * state, to be saved and loaded with the weights.  Table and stream as above.
+ * state, to be saved and loaded with the weights (each plan has its own).  Table and stream as above.
+ * Buffers that overlap are refused: a weight that two layers share is listed once.
  * With states in 8 bits expAvg holds e4m3 codes (1 sign, 4 exponent, 3 fraction bits, largest 448) of
  * m / scale, and expAvgSq of sqrt(v) / scale, scale = the run's largest magnitude / 448; a second
  * moment above zero never gets the zero code (its step would be m / eps).  Codes and scales of zero
@@ -96,6 +97,7 @@ ncclResult_t mscclAmdAdamWSetGrads(mscclAmdAdamW_t plan, const void* const* grad
  *   c = gradScale, and with a square sum and maxNorm > 0 times min(1, maxNorm / (norm + 1e-6)),
  *   norm = gradScale * sqrt(*gradSquareSum).
  * A square sum that is not finite leaves everything as it was, step included.
+ * eps and gradScale are normal 32-bit values (eps may be 0), the betas in [0, 1).
  *   lrDevice       NULL, or a 32-bit learning rate on the device in place of lr (a captured step
  *                  follows a schedule through it)
  *   gradSquareSum  NULL, or the square sum of the gradients as they are, over all ranks
@@ -144,7 +146,8 @@ ncclResult_t mscclAmdBalanceLoss(const int64_t* counts, const float* probs, size
  * grad[t][e] = gradLoss * dloss / dx, zero in padded rows (type and shape as logits).
  *   gradLoss    NULL (1), or one 32-bit value
  *   accumulate  nonzero: added to what grad holds, in 32 bits, and rounded once; padded rows stay
- * router->index, indexType, indexStride are not used.  grad may be logits itself without accumulate. */
+ * router->index, indexType, indexStride are not used.  grad may be logits itself without accumulate;
+ * otherwise no element of the two is the same. */
 ncclResult_t mscclAmdBalanceBackward(const mscclAmdRouter_t* router, const int64_t* counts, double coef,
                                      const float* gradLoss, void* grad, size_t gradStride, int accumulate,
                                      hipStream_t stream);

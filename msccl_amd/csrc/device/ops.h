@@ -14,7 +14,7 @@ constexpr int kStateBlock = 256;     // elements that share a scale in 8-bit sta
 // (AdamW: `wide`, where a tensor beside 8-bit states is in 32 bits)
 constexpr int adamEach(int bits, bool wide) { return bits == 8 && wide ? 4 : 8; }   // elements a lane
 constexpr uint32_t adamChunk(int bits, bool wide) { return kOpsThreads * adamEach(bits, wide); }
-constexpr int kSumVecs = 4;          // 16-byte vectors a lane
+constexpr int kSumVecs = 2;          // 16-byte vectors a lane
 constexpr uint32_t sumChunk(size_t elemSize) { return kOpsThreads * (16 / elemSize) * kSumVecs; }
 
 // rows of the tensor tables; a table is [rows][starts: n + 1 chunk numbers, uint32_t]
@@ -97,7 +97,11 @@ int balanceBlocks(int64_t tokens, int experts);   // workgroups of the statistic
 int launchBalanceStats(const BalanceArgs& a, int type, bool index64, bool sigmoid, int blocks, void* stream);
 int launchBalanceLoss(const int64_t* counts, const float* probs, int experts, double scale, float* loss, void* stream);
 int launchBalanceBackward(const BalanceArgs& a, int type, bool sigmoid, bool accumulate, void* stream);
-constexpr int kSumBlocks = 2048;        // most workgroups (partial sums) of a square sum
+constexpr int kSumThreads = 1024;       // a workgroup of a square sum: four groups that take chunks by themselves
+constexpr int kSumBlocks = 256;         // most of them, and of the partial sums
+// Up to this many chunks one workgroup and one launch: 65536 32-bit values 5.3 us, with the second launch 9.5
+// (both the host's time); 131072 would take the workgroup longer than the host.
+constexpr uint32_t kSumOne = 32;
 constexpr int kMaxExperts = 1024;
 
 }  // namespace msccl
@@ -241,6 +245,20 @@ __device__ __forceinline__ float sumOver(float x) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
   }));
 }
+// a wave's sum of 64-bit values: the halves exchanged alike
+__device__ __forceinline__ double waveSum(double x) {
+  const auto add = [](double a, uint32_t hi, uint32_t lo) { return a + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };
+#define OPS_STEP(CTRL) do { const uint64_t b = __builtin_bit_cast(uint64_t, x); \
+    x = add(x, dpp<CTRL>((uint32_t)(b >> 32)), dpp<CTRL>((uint32_t)b)); } while (0)
+  OPS_STEP(0xB1);
+  OPS_STEP(0x4E);
+  OPS_STEP(0x141);
+  OPS_STEP(0x140);
+#undef OPS_STEP
+  x += __shfl_xor(x, 16);
+  x += __shfl_xor(x, 32);
+  return x;
+}
 template <int L>
 __device__ __forceinline__ uint32_t umaxOver(uint32_t x) {
   return reduceLanes<L>(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
@@ -248,33 +266,36 @@ __device__ __forceinline__ uint32_t umaxOver(uint32_t x) {
 
 // The tensor that chunk c of a table lies in: the last row whose first chunk is at most c (empty
 // tensors start where the next one does).  All lanes of a wave look at once, 64 rows apart in each
-// round: one round for 64 tensors, two for 4096.
-__device__ __forceinline__ uint32_t findTensor(const uint32_t* starts, uint32_t n, uint32_t c) {
+// round: one round for 64 tensors, two for 4096.  What the first round compares is the same for every
+// chunk: searchStart, read once.
+__device__ __forceinline__ uint32_t searchStart(const uint32_t* starts, uint32_t n) {
+  const uint32_t i = (threadIdx.x & 63) * ((n + 63) / 64);
+  return i < n ? inGlobal(starts)[i] : 0xffffffffu;
+}
+__device__ __forceinline__ uint32_t findTensor(const uint32_t* starts, uint32_t n, uint32_t c, uint32_t seen) {
   uint32_t lo = 0, len = n;
   const uint32_t lane = threadIdx.x & 63;
   while (len > 1) {
     const uint32_t step = (len + 63) / 64;
-    const uint32_t i = lane * step;
-    const bool below = i < len && inGlobal(starts)[lo + i] <= c;
-    const uint32_t k = __builtin_popcountll(__ballot(below)) - 1;
+    const uint32_t k = __builtin_popcountll(__ballot(seen <= c)) - 1;
     lo += k * step;
     const uint32_t left = len - k * step;
     len = left < step ? left : step;
+    if (len > 1) {
+      const uint32_t i = lane * ((len + 63) / 64);
+      seen = i < len ? inGlobal(starts)[lo + i] : 0xffffffffu;
+    }
   }
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-template <class T>
-__device__ __forceinline__ T blockSum(T x, T* lds) {   // every thread gets the sum; lds: one T a wave
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
-  const int waves = blockDim.x / 64;
+// The workgroup's sum (thread 0's): the wave's by exchanges, the waves' by LDS (lds: one value a wave).
+template <int WAVES>
+__device__ __forceinline__ double blockSum(double x, double* lds) {
+  x = waveSum(x);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x / 64] = x;
   __syncthreads();
-  T s = lds[0];
-  for (int w = 1; w < waves; w++) s += lds[w];
-  __syncthreads();
-  return s;
+  return threadIdx.x < 64 ? waveSum(threadIdx.x < WAVES ? lds[threadIdx.x] : 0.0) : 0.0;
 }
 
 }  // namespace msccl

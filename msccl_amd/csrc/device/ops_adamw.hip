@@ -286,8 +286,9 @@ __global__ void __launch_bounds__(kOpsThreads) adamwKernel(AdamStepArgs a) {
   }
   if (ctl.skip) return;
   constexpr uint32_t chunk = adamChunk(BITS, MASTER || sizeof(P) == 4 || sizeof(G) == 4);
+  const uint32_t seen = searchStart(a.tab.starts, a.tab.n);
   for (uint32_t c = blockIdx.x; c < a.tab.chunks; c += gridDim.x) {
-    const uint32_t ti = findTensor(a.tab.starts, a.tab.n, c);
+    const uint32_t ti = findTensor(a.tab.starts, a.tab.n, c, seen);
     const AdamTensor* t = a.tab.rows + ti;
     const uint64_t from = (uint64_t)(c - scalarLoad(a.tab.starts + ti)) * chunk;
     const uint64_t left = scalarLoad(&t->count) - from;

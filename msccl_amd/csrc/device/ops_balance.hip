@@ -170,9 +170,15 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
       if ((uint64_t)e[k] < (uint64_t)a.experts) atomicAdd(&hist[copies == 1 ? 0 : wave][e[k]], 1u);
   }
 
+  // 64 rows at most are added up in 32 bits; those sums in 64
   f32x8 acc[VPL];
+  double total[VPL][8];
 #pragma unroll
-  for (int j = 0; j < VPL; j++) acc[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};
+  for (int j = 0; j < VPL; j++) {
+    acc[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++) total[j][i] = 0.0;
+  }
   uint32_t here = 0;
   for (int r = own; r < rows; r += rowsPer) {
     f32x8 x[VPL];
@@ -193,6 +199,20 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
     for (int j = 0; j < VPL; j++)
 #pragma unroll
       for (int i = 0; i < 8; i++) acc[j][i] = fmaf(x[j][i], inv, acc[j][i]);
+    if (here % 64 == 0) {
+#pragma unroll
+      for (int j = 0; j < VPL; j++) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) total[j][i] += (double)acc[j][i];
+        acc[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};
+      }
+    }
+  }
+  if (here >= 64) {
+#pragma unroll
+    for (int j = 0; j < VPL; j++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) acc[j][i] = (float)(total[j][i] + (double)acc[j][i]);
   }
   if (here && lane == 0) atomicAdd(&tokens, here);
   // over the wave's rows, then over the waves: the upper half's on top of the lower half's
@@ -288,7 +308,7 @@ __global__ void __launch_bounds__(kOpsThreads) balanceLossKernel(const int64_t* 
   __shared__ double lds[kOpsThreads / 64];
   double s = 0.0;
   for (int e = threadIdx.x; e < experts; e += kOpsThreads) s += (double)counts[e] * (double)probs[e];
-  s = blockSum(s, lds);
+  s = blockSum<kOpsThreads / 64>(s, lds);
   if (threadIdx.x == 0) {
     const double n = (double)counts[experts];
     *loss = n > 0 ? (float)(s * scale / (n * n)) : 0.f;

@@ -9,24 +9,27 @@
 namespace msccl {
 
 template <class T>
-__global__ void __launch_bounds__(kOpsThreads) squareSumKernel(TensorTable<SumTensor> tab, double* partials) {
-  __shared__ double lds[kOpsThreads / 64];
+__global__ void __launch_bounds__(kSumThreads) squareSumKernel(TensorTable<SumTensor> tab, double* partials) {
+  __shared__ double lds[kSumThreads / 64];
+  constexpr uint32_t groups = kSumThreads / kOpsThreads;
+  const uint32_t group = __builtin_amdgcn_readfirstlane(threadIdx.x / kOpsThreads), lane = threadIdx.x % kOpsThreads;
   constexpr int N = 16 / sizeof(T);
   constexpr uint32_t chunk = sumChunk(sizeof(T));
   double s = 0.0;
-  for (uint32_t c = blockIdx.x; c < tab.chunks; c += gridDim.x) {
-    const uint32_t ti = findTensor(tab.starts, tab.n, c);
+  const uint32_t seen = searchStart(tab.starts, tab.n);
+  for (uint32_t c = blockIdx.x * groups + group; c < tab.chunks; c += gridDim.x * groups) {
+    const uint32_t ti = findTensor(tab.starts, tab.n, c, seen);
     const uint64_t from = (uint64_t)(c - scalarLoad(tab.starts + ti)) * chunk;
     const uint64_t left = scalarLoad(&tab.rows[ti].count) - from;
     const T* data = (const T*)scalarLoad(&tab.rows[ti].data) + from;
     typename VecOf<T, N>::F x[kSumVecs];
     if (left >= chunk) {
 #pragma unroll
-      for (int j = 0; j < kSumVecs; j++) x[j] = loadN<N>(data + (j * kOpsThreads + threadIdx.x) * N, N);
+      for (int j = 0; j < kSumVecs; j++) x[j] = loadN<N>(data + (j * kOpsThreads + lane) * N, N);
     } else {
 #pragma unroll
       for (int j = 0; j < kSumVecs; j++) {
-        const uint32_t mine = (j * kOpsThreads + threadIdx.x) * N;
+        const uint32_t mine = (j * kOpsThreads + lane) * N;
         x[j] = loadN<N>(data + mine, (int)left - (int)mine);
       }
     }
@@ -35,30 +38,24 @@ __global__ void __launch_bounds__(kOpsThreads) squareSumKernel(TensorTable<SumTe
 #pragma unroll
       for (int i = 0; i < N; i++) s = fma((double)x[j][i], (double)x[j][i], s);
   }
-  s = blockSum(s, lds);
+  s = blockSum<kSumThreads / 64>(s, lds);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
 }
 
-__global__ void __launch_bounds__(1024) sumPartialsKernel(const double* partials, int n, double* out) {
-  __shared__ double lds[16];
-  double s = 0.0;
-#pragma unroll
-  for (int k = 0; k < kSumBlocks / 1024; k++) {
-    const int i = k * 1024 + threadIdx.x;
-    s += i < n ? partials[i] : 0.0;
-  }
-  s = blockSum(s, lds);
+__global__ void __launch_bounds__(kSumBlocks) sumPartialsKernel(const double* partials, int n, double* out) {
+  __shared__ double lds[kSumBlocks / 64];
+  const double s = blockSum<kSumBlocks / 64>((int)threadIdx.x < n ? partials[threadIdx.x] : 0.0, lds);
   if (threadIdx.x == 0) *out = s;
 }
 
 template <class T>
 static int launchSum(const TensorTable<SumTensor>& tab, double* out, double* partials, int blocks, void* stream) {
   // one workgroup's partial sum is the sum
-  hipLaunchKernelGGL(squareSumKernel<T>, dim3(blocks), dim3(kOpsThreads), 0, (hipStream_t)stream, tab,
+  hipLaunchKernelGGL(squareSumKernel<T>, dim3(blocks), dim3(kSumThreads), 0, (hipStream_t)stream, tab,
                      blocks == 1 ? out : partials);
   if (hipGetLastError() != hipSuccess) return 1;
   if (blocks == 1) return 0;
-  hipLaunchKernelGGL(sumPartialsKernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, partials, blocks, out);
+  hipLaunchKernelGGL(sumPartialsKernel, dim3(1), dim3(kSumBlocks), 0, (hipStream_t)stream, partials, blocks, out);
   return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 

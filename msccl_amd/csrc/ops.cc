@@ -1,8 +1,11 @@
 // Training-step operators: argument checks, plans and launches (include/msccl_amd_ops.h).
-#include <cmath>
 #include <string.h>
 
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include <hip/hip_runtime.h>
@@ -61,6 +64,18 @@ TensorTable<Row> tableAt(void* device, size_t n, uint32_t chunks) {
 
 constexpr size_t kMostTensors = 1u << 20;
 
+typedef std::pair<uintptr_t, uintptr_t> Range;   // first address, and the one behind the last
+
+void addRange(std::vector<Range>* to, const void* p, size_t bytes) {
+  if (p && bytes) to->push_back(Range((uintptr_t)p, (uintptr_t)p + bytes));
+}
+
+// whether r meets one of these (sorted, apart from each other)
+bool meets(const std::vector<Range>& sorted, const Range& r) {
+  const auto after = std::lower_bound(sorted.begin(), sorted.end(), Range(r.second, 0));
+  return after != sorted.begin() && (after - 1)->second > r.first;
+}
+
 }  // namespace
 
 struct mscclAmdSquareSumPlan {
@@ -79,6 +94,7 @@ struct mscclAmdAdamWPlan {
   AdamTensor* rows;
   TensorTable<AdamTensor> tab;
   std::vector<size_t> counts;
+  std::vector<Range> written;   // sorted
 };
 
 extern "C" {
@@ -112,7 +128,9 @@ ncclResult_t mscclAmdSquareSumCreate(mscclAmdSquareSum_t* plan, const void* cons
       WARN("%s : launch failed", name);
       return ncclUnhandledCudaError;
     }
-    const int blocks = chunks <= 1 ? 1 : chunks < (uint32_t)kSumBlocks ? (int)chunks : kSumBlocks;
+    constexpr uint32_t groups = kSumThreads / kOpsThreads;
+    const uint32_t wanted = chunks <= kSumOne ? 1 : (chunks + groups - 1) / groups;
+    const int blocks = wanted < (uint32_t)kSumBlocks ? (int)wanted : kSumBlocks;
     *plan = new mscclAmdSquareSumPlan{kSumMagic, (int)type, blocks, tableAt<SumTensor>(device, n, chunks)};
   } catch (const std::bad_alloc&) {
     WARN("%s : out of host memory", name);
@@ -192,6 +210,26 @@ ncclResult_t mscclAmdAdamWCreate(mscclAmdAdamW_t* plan, const mscclAmdAdamWTenso
       if (!std::isfinite(t.weightDecay) || !std::isfinite(t.lrScale)) REFUSE("%s : tensor %zu: decay or lrScale is not finite", name, i);
       rows[i] = AdamTensor{t.param, t.grad, t.master, t.expAvg, t.expAvgSq, t.expAvgScale, t.expAvgSqScale, t.count, t.weightDecay, t.lrScale};
     }
+    // what a step writes lies apart, from itself and from the gradients
+    std::vector<Range> written;
+    written.reserve(6 * n + 1);
+    addRange(&written, step, 8);
+    for (const AdamTensor& t : rows) {
+      if (t.count > (size_t)1 << 60) REFUSE("%s : too many elements", name);
+      const size_t runs = (t.count + kStateBlock - 1) / kStateBlock;
+      addRange(&written, t.param, t.count * ps);
+      addRange(&written, t.master, t.count * 4);
+      addRange(&written, t.m, t.count * (stateBits / 8));
+      addRange(&written, t.v, t.count * (stateBits / 8));
+      addRange(&written, t.mScale, runs * 4);
+      addRange(&written, t.vScale, runs * 4);
+    }
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); i++)
+      if (written[i - 1].second > written[i].first) REFUSE("%s : buffers overlap (a tensor twice?)", name);
+    for (size_t i = 0; i < n; i++)
+      if (rows[i].count && meets(written, Range((uintptr_t)rows[i].grad, (uintptr_t)rows[i].grad + rows[i].count * gs)))
+        REFUSE("%s : gradient %zu overlaps what the step writes", name, i);
     std::vector<uint64_t> image;
     uint32_t chunks;
     if (!makeTable(&image, rows.data(), n, adamChunk(stateBits, master || ps == 4 || gs == 4), &chunks)) REFUSE("%s : too many elements", name);
@@ -203,7 +241,7 @@ ncclResult_t mscclAmdAdamWCreate(mscclAmdAdamW_t* plan, const mscclAmdAdamWTenso
       return ncclUnhandledCudaError;
     }
     *plan = new mscclAmdAdamWPlan{kAdamMagic, (int)paramType, (int)gradType, stateBits, master, step, (AdamControl*)device,
-                              (AdamTensor*)table, tableAt<AdamTensor>(table, n, chunks), std::move(counts)};
+                              (AdamTensor*)table, tableAt<AdamTensor>(table, n, chunks), std::move(counts), std::move(written)};
   } catch (const std::bad_alloc&) {
     WARN("%s : out of host memory", name);
     return ncclSystemError;
@@ -218,7 +256,10 @@ ncclResult_t mscclAmdAdamWSetGrads(mscclAmdAdamW_t plan, const void* const* grad
   if (n && !grads) REFUSE("%s : gradient list is NULL", name);
   for (size_t i = 0; i < n; i++) {
     if (plan->counts[i] && !grads[i]) REFUSE("%s : gradient %zu is NULL", name, i);
-    if (!aligned(grads[i], elemSize(plan->gradType))) REFUSE("%s : gradient %zu is not aligned to its elements", name, i);
+    const size_t gs = elemSize(plan->gradType);
+    if (!aligned(grads[i], gs)) REFUSE("%s : gradient %zu is not aligned to its elements", name, i);
+    if (plan->counts[i] && meets(plan->written, Range((uintptr_t)grads[i], (uintptr_t)grads[i] + plan->counts[i] * gs)))
+      REFUSE("%s : gradient %zu overlaps what the step writes", name, i);
   }
   if (launchGradWrite(plan->rows, grads, n, stream)) {
     WARN("%s : launch failed", name);
@@ -234,8 +275,8 @@ ncclResult_t mscclAmdAdamWStep(mscclAmdAdamW_t plan, double lr, const float* lrD
   if (!plan || plan->magic != kAdamMagic) REFUSE("%s : invalid plan", name);
   if (!std::isfinite(lr)) REFUSE("%s : lr is not finite", name);
   if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1)) REFUSE("%s : betas (%g, %g) outside [0, 1)", name, beta1, beta2);
-  if (!(eps >= 0) || !std::isfinite(eps)) REFUSE("%s : eps %g", name, eps);
-  if (!(gradScale > 0) || !std::isfinite(gradScale)) REFUSE("%s : gradScale %g is not above zero", name, gradScale);
+  if (!(eps == 0 || (eps >= FLT_MIN && eps <= FLT_MAX))) REFUSE("%s : eps %g (0, or a normal 32-bit value)", name, eps);
+  if (!(gradScale >= FLT_MIN && gradScale <= FLT_MAX)) REFUSE("%s : gradScale %g (a normal 32-bit value above zero)", name, gradScale);
   if (!(maxNorm >= 0)) REFUSE("%s : maxNorm %g", name, maxNorm);
   if (maxNorm > 0 && !gradSquareSum) REFUSE("%s : maxNorm without a square sum", name);
   if (!aligned(gradSquareSum, 8) || !aligned(lrDevice, 4)) REFUSE("%s : gradSquareSum or lrDevice is not aligned", name);
@@ -280,6 +321,7 @@ static ncclResult_t checkRouter(const char* name, const mscclAmdRouter_t* r, boo
   if (r->experts < 1 || r->experts > (size_t)kMaxExperts) REFUSE("%s : %zu experts (1 to %d)", name, r->experts, kMaxExperts);
   if (r->topK < 1 || r->topK > r->experts) REFUSE("%s : topK %zu of %zu experts", name, r->topK, r->experts);
   if (r->tokens > (size_t)1 << 30) REFUSE("%s : %zu tokens, at most 2^30", name, r->tokens);
+  if (r->tokens * r->topK > (size_t)1 << 39) REFUSE("%s : %zu slots, at most 2^39", name, r->tokens * r->topK);
   if (r->logitStride < r->experts || r->logitStride > (size_t)1 << 30) REFUSE("%s : logitStride %zu", name, r->logitStride);
   if (r->tokens && !r->logits) REFUSE("%s : logits is NULL", name);
   if (!aligned(r->logits, es)) REFUSE("%s : logits is not aligned to its elements", name);

@@ -25,13 +25,8 @@ _SCORES = {"softmax": 0, "sigmoid": 1}
 STATE_BLOCK = 256  # elements that share a scale in 8-bit states
 
 
-class _AdamWTensor(ctypes.Structure):
-    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("master", ctypes.c_void_p),
-                ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
-                ("exp_avg_scale", ctypes.c_void_p), ("exp_avg_sq_scale", ctypes.c_void_p),
-                ("count", ctypes.c_size_t), ("weight_decay", ctypes.c_double), ("lr_scale", ctypes.c_double)]
-
-
+# mscclAmdAdamWTensor_t: param, grad, master, expAvg, expAvgSq, expAvgScale, expAvgSqScale, count, weightDecay, lrScale
+_TENSOR = struct.Struct("@PPPPPPPNdd")
 # mscclAmdRouter_t: logits, type, tokens, experts, logitStride, index, indexType, topK, indexStride, valid, score
 _ROUTER = struct.Struct("@PiNNNPiNNPi")
 
@@ -53,7 +48,7 @@ def _lib():
         L.mscclAmdSquareSumDestroy.argtypes = [vp]
         L.mscclAmdAdamWBytes.argtypes = [sz]
         L.mscclAmdAdamWBytes.restype = sz
-        L.mscclAmdAdamWCreate.argtypes = [ctypes.POINTER(vp), vp, sz, i, i, i, vp, vp, sz, vp]
+        L.mscclAmdAdamWCreate.argtypes = [ctypes.POINTER(vp), ctypes.c_char_p, sz, i, i, i, vp, vp, sz, vp]
         L.mscclAmdAdamWSetGrads.argtypes = [vp, vp, sz, vp]
         L.mscclAmdAdamWStep.argtypes = [vp, d, vp, d, d, d, d, vp, d, vp]
         L.mscclAmdAdamWDestroy.argtypes = [vp]
@@ -76,8 +71,13 @@ def _elsewhere(device) -> bool:
     return torch._C._cuda_getDevice() != device.index
 
 
-def _flat(t, what: str, dtypes, device=None, numel: Optional[int] = None) -> None:
+def _flat(t, what: str, dtypes, device=None, numel: Optional[int] = None, i: Optional[int] = None) -> None:
     """A contiguous device tensor of one of `dtypes`, or an exception."""
+    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.is_contiguous() and
+            (device is None or t.device == device) and (numel is None or t.numel() == numel)):
+        return
+    if i is not None:
+        what = "%s[%d]" % (what, i)
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch tensor" % what)
     if t.device.type != "cuda":
@@ -88,8 +88,17 @@ def _flat(t, what: str, dtypes, device=None, numel: Optional[int] = None) -> Non
         raise ValueError("%s must be contiguous" % what)
     if device is not None and t.device != device:
         raise ValueError("%s is on %s, not %s" % (what, t.device, device))
-    if numel is not None and t.numel() != numel:
-        raise ValueError("%s has %d elements, not %d" % (what, t.numel(), numel))
+    raise ValueError("%s has %d elements, not %d" % (what, t.numel(), numel))
+
+
+def _span(tensors):
+    """The first address of these tensors and the one behind the last (None: they are all empty)."""
+    ends = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in tensors if t.numel()]
+    return (min(a for a, _ in ends), max(b for _, b in ends)) if ends else None
+
+
+def _inside(span, at: int, nbytes: int) -> bool:
+    return span is None or (at <= span[0] and span[1] <= at + nbytes)
 
 
 class _Plan:
@@ -104,14 +113,20 @@ class _Plan:
             raise RuntimeError("make the plan before the capture")
         self.device = device
         self.table = torch.empty(max(8, nbytes), dtype=torch.uint8, device=device)
+        self._home = _stream(device)
 
     def _ready(self):
         # the table was written on this stream; the plan may be used on any
         torch.cuda.current_stream(self.device).synchronize()
 
-    def _live(self):
+    def _live(self) -> int:
+        """The stream of a call on the plan."""
         if not self.handle:
             raise ValueError("the plan is closed")
+        s = _stream(self.device)
+        if s != self._home:  # the table's memory is not to be used again before this stream is done with it
+            self.table.record_stream(torch.cuda.current_stream(self.device))
+        return s
 
     def close(self) -> None:
         """Ends the plan.  The device must be done with its calls."""
@@ -140,8 +155,10 @@ class SquareSum(_Plan):
         if not self.tensors:
             raise ValueError("no tensors")
         first = self.tensors[0]
+        dev = getattr(first, "device", None)
+        dtypes = (first.dtype,) if getattr(first, "dtype", None) in _TYPES else tuple(_TYPES)
         for i, t in enumerate(self.tensors):
-            _flat(t, "tensor %d" % i, (first.dtype,) if first.dtype in _TYPES else tuple(_TYPES), self.tensors[0].device)
+            _flat(t, "tensors", dtypes, dev, None, i)
         n = len(self.tensors)
         L = _lib()
         with torch.cuda.device(first.device):
@@ -153,9 +170,10 @@ class SquareSum(_Plan):
                    "mscclAmdSquareSumCreate")
             self._ready()
         self._scratch = L.mscclAmdSquareSumWorkspace(self.handle)
+        self.span = _span(self.tensors)
 
     def __call__(self, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        self._live()
+        stream = self._live()
         if out is not None:
             _flat(out, "out", (torch.float64,), self.device, 1)
         dev = self.device
@@ -167,7 +185,7 @@ class SquareSum(_Plan):
         if out is None:
             out = torch.empty(1, dtype=torch.float64, device=dev)
         rc = _lib().mscclAmdSquareSum(self.handle, out.data_ptr(), scratch.data_ptr() if self._scratch else None,
-                                      self._scratch, _stream(dev))
+                                      self._scratch, stream)
         if rc:
             raise NcclError(rc, "mscclAmdSquareSum")
         return out
@@ -197,9 +215,10 @@ class AdamW(_Plan):
     params and grads: contiguous, one type each (float32, float16, bfloat16); masters: None, or the
     weights in float32 (read in place of params, both are written).  exp_avgs, exp_avg_sqs: float32, or
     torch.float8_e4m3fn with exp_avg_scales and exp_avg_sq_scales, one float32 for each 256 elements of
-    a tensor (the last may be shorter); adamw_state makes them.  step: one int64, the steps taken so far.
-    weight_decay, lr_scale: a number, or one for each tensor.  Tensors may have any size and start
-    anywhere; they must not overlap.  Steps of one plan must be ordered after each other."""
+    a tensor (the last may be shorter); adamw_state makes them.  step: one int64, the steps taken so far,
+    this plan's own.  weight_decay, lr_scale: a number, or one for each tensor.  Tensors may have any size
+    and start anywhere; they must not overlap (a weight that layers share is listed once).  Steps of one
+    plan must be ordered after each other."""
     _destroy = "mscclAmdAdamWDestroy"
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
@@ -230,8 +249,8 @@ class AdamW(_Plan):
                 continue
             if len(ts) != n:
                 raise ValueError("%d %s for %d tensors" % (len(ts), what, n))
-            for i, t in enumerate(ts):
-                _flat(t, "%s[%d]" % (what, i), dtypes, dev, -(-params[i].numel() // per))
+            for i, (t, p) in enumerate(zip(ts, params)):
+                _flat(t, what, dtypes, dev, -(-p.numel() // per), i)
         if len(decay) != n or len(rates) != n:
             raise ValueError("weight_decay and lr_scale: a number, or one for each tensor")
         if any(g.dtype != grads[0].dtype for g in grads):
@@ -239,12 +258,10 @@ class AdamW(_Plan):
         _flat(step, "step", (torch.int64,), dev, 1)
         self.tensors = [list(ts) if ts is not None else None for _, ts, _, _ in lists] + [step]
         self._grad_type = grads[0].dtype
-        rows = (_AdamWTensor * n)()
-        for i in range(n):
-            r = rows[i]
-            r.param, r.grad, r.master, r.exp_avg, r.exp_avg_sq, r.exp_avg_scale, r.exp_avg_sq_scale = [
-                ts[i].data_ptr() if ts is not None else None for _, ts, _, _ in lists]
-            r.count, r.weight_decay, r.lr_scale = params[i].numel(), float(decay[i]), float(rates[i])
+        self.param_span, self.grad_span = _span(params), _span(grads)
+        at = [[t.data_ptr() for t in ts] if ts is not None else [0] * n for _, ts, _, _ in lists]
+        rows = b"".join(_TENSOR.pack(*row, t.numel(), float(d), float(r))
+                        for *row, t, d, r in zip(*at, params, decay, rates))
         L = _lib()
         with torch.cuda.device(dev):
             self._memory(dev, L.mscclAmdAdamWBytes(n))
@@ -256,7 +273,7 @@ class AdamW(_Plan):
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
         """Other gradient tensors (same sizes and type) for the steps enqueued from now on; the earlier
         steps must be on the current stream or ordered before it."""
-        self._live()
+        stream = self._live()
         params = self.tensors[0]
         if len(grads) != len(params):
             raise ValueError("%d gradients for %d tensors" % (len(grads), len(params)))
@@ -264,9 +281,9 @@ class AdamW(_Plan):
             _flat(g, "grads[%d]" % i, (self._grad_type,), self.device, params[i].numel())
         ptrs = (ctypes.c_void_p * len(grads))(*[g.data_ptr() for g in grads])
         with torch.cuda.device(self.device):
-            _check(_lib().mscclAmdAdamWSetGrads(self.handle, ptrs, len(grads), _stream(self.device)),
-                   "mscclAmdAdamWSetGrads")
+            _check(_lib().mscclAmdAdamWSetGrads(self.handle, ptrs, len(grads), stream), "mscclAmdAdamWSetGrads")
         self.tensors[1] = list(grads)
+        self.grad_span = _span(grads)
 
     def step(self, lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8, grad_scale: float = 1.0,
              grad_square_sum: Optional[torch.Tensor] = None, max_norm: Optional[float] = None) -> None:
@@ -274,7 +291,7 @@ class AdamW(_Plan):
         which a captured step reads at each replay.  grad_scale: a factor on the gradients (one over the
         ranks that were summed, or over a loss scale).  grad_square_sum: the square sum of the gradients as
         they are, over all ranks; if it is not finite the step changes nothing.  max_norm: clips to it."""
-        self._live()
+        stream = self._live()
         at = None
         if isinstance(lr, torch.Tensor):
             _flat(lr, "lr", (torch.float32,), self.device, 1)
@@ -286,7 +303,7 @@ class AdamW(_Plan):
         if max_norm is not None and not max_norm > 0:
             raise ValueError("max_norm must be above zero")
         launch, args = _lib().mscclAmdAdamWStep, (self.handle, lr, at, betas[0], betas[1], eps, grad_scale, total,
-                                                  max_norm or 0.0, _stream(self.device))
+                                                  max_norm or 0.0, stream)
         if _elsewhere(self.device):
             with torch.cuda.device(self.device):
                 rc = launch(*args)
@@ -321,6 +338,12 @@ def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: S
             raise ValueError("the shards must have one size and type")
         if plans[r].device != dev or sums[r].device != dev:
             raise ValueError("plans[%d] or sums[%d] is on another device than its communicator" % (r, r))
+        size = block * shards[r].element_size()
+        if not (_inside(plans[r].grad_span, shards[r].data_ptr(), size) and _inside(sums[r].span, shards[r].data_ptr(), size)):
+            raise ValueError("plans[%d] or sums[%d] reads gradients outside shards[%d]" % (r, r, r))
+        size = block * params[r].element_size()
+        if not _inside(plans[r].param_span, params[r].data_ptr() + c.rank * size, size):
+            raise ValueError("plans[%d] writes weights outside its rank's block of params[%d]" % (r, r))
     block, es = shards[0].numel(), params[0].element_size()
     gt, pt = _TYPES[shards[0].dtype], _TYPES[params[0].dtype]
     with group():

@@ -415,6 +415,7 @@ def test_adamw_refuses():
     bad = [dict(grads=g[:1]), dict(grads=[g[0], g[0]]), dict(grads=[g[0], g[1].double()]), dict(grads=[g[0], g[1].bfloat16()]),
            dict(step=s.int()), dict(step=s.cpu()), dict(masters=[x.clone() for x in p]), dict(exp_avg_scales=[s.float()] * 2),
            dict(exp_avgs=[x.to(E4M3) for x in m]), dict(exp_avgs=[x.double() for x in m]), dict(weight_decay=[0.1]),
+           dict(params=[p[1][:10], p[1]]), dict(grads=[p[0], g[1]]), dict(exp_avgs=[m[0], v[1]]),
            dict(params=[x.double() for x in p]), dict(lr_scale=[1.0] * 3)]
     for kw in bad:
         args = dict(params=p, grads=g, exp_avgs=m, exp_avg_sqs=v, step=s) | kw
@@ -422,7 +423,7 @@ def test_adamw_refuses():
             ops.AdamW(**args)
     old = k.copy()
     total = torch.ones(1, dtype=torch.float64, device="cuda")
-    for kw in [dict(lr=float("nan")), dict(betas=(1.0, 0.9)), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(eps=-1.0),
+    for kw in [dict(lr=float("nan")), dict(betas=(1.0, 0.9)), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(eps=-1.0), dict(eps=1e-40), dict(grad_scale=1e39),
                dict(eps=float("inf")), dict(grad_scale=0.0), dict(grad_scale=-1.0), dict(grad_scale=float("inf")),
                dict(max_norm=1.0), dict(max_norm=0.0, grad_square_sum=total), dict(max_norm=-1.0, grad_square_sum=total),
                dict(grad_square_sum=total.float()), dict(grad_square_sum=total.cpu()), dict(lr=s)]:
@@ -432,6 +433,8 @@ def test_adamw_refuses():
         k.plan.set_grads(g[:1])
     with pytest.raises(ValueError):
         k.plan.set_grads([g[1], g[0]])
+    with pytest.raises(ops.NcclError):
+        k.plan.set_grads([g[0], m[1]])
     torch.cuda.synchronize()
     assert k.same(old)
     k.plan.close()
@@ -642,6 +645,30 @@ def test_balance_one_expert_takes_all():
     assert int(counts[17]) == 300_000
 
 
+def test_balance_many_rows_a_lane():
+    # a lane adds up 300 rows: its sums of 64 rows go on in 64 bits (what the plain bound of 81 counts)
+    logits, ind, valid = router(256 * 16 * 300, 500, 2, F16, False)
+    check_stats(logits, ind, torch.ones(len(ind), dtype=torch.bool, device="cuda"), "softmax")
+
+
+def test_plans_on_other_streams_keep_their_tables():
+    # a plan that is dropped while another stream still has its calls to make
+    x = torch.randn(1 << 22, device="cuda")
+    want = ops.SquareSum([x])()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        plan = ops.SquareSum([x])
+        with torch.cuda.stream(side):
+            for _ in range(50):
+                got = plan()
+        del plan
+        junk = [torch.full((64,), 255, dtype=torch.uint8, device="cuda") for _ in range(20)]
+        side.synchronize()
+        assert torch.equal(got, want)
+        del junk
+
+
 def test_balance_far_rows():
     # rows whose elements lie past 2^31 of the buffer
     rows, stride = 9, (1 << 28) + 8
@@ -816,3 +843,9 @@ def run_sharded(comms, bits):
         ops.sharded_step(comms, bad, shards, params, plans, sums[:1], lr=1e-2)
     with pytest.raises(ValueError):
         ops.sharded_step(comms, [g[:-1] for g in bad], shards, params, plans, sums, lr=1e-2)
+    with pytest.raises(ValueError):
+        ops.sharded_step(comms, bad, [s.clone() for s in shards], params, plans, sums, lr=1e-2)
+    with pytest.raises(ValueError):
+        ops.sharded_step(comms, bad, shards, [p.clone() for p in params], plans, sums, lr=1e-2)
+    with pytest.raises(ValueError):
+        ops.sharded_step(comms, bad, shards, params, plans[::-1], sums, lr=1e-2)

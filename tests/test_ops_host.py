@@ -41,16 +41,20 @@ def test_square_sum_refuses_bad_plan():
     assert L.mscclAmdSquareSumDestroy(ctypes.addressof(junk)) == BAD
 
 
-def adamw_create(tensor=None, n=1, paramType=F32, gradType=F32, bits=32, step=A, device=A, nbytes=1 << 16, plan=True,
+TENSOR_FIELDS = ("param", "grad", "master", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "count",
+                 "weight_decay", "lr_scale")
+
+
+def adamw_create(tensor=None, n=1, paramType=F32, gradType=F32, bits=32, step=7 * A, device=8 * A, nbytes=1 << 16, plan=True,
                  second=None):
     L = ops._lib()
-    rows = (ops._AdamWTensor * 2)()
-    for i, over in enumerate((tensor or {}, (tensor or {}) if second is None else second)):
-        base = dict(param=A, grad=A, exp_avg=A, exp_avg_sq=A, count=10, lr_scale=1.0)
+    rows = b""
+    for over in (tensor or {}, (tensor or {}) if second is None else second):
+        o = 4096 * len(rows)
+        base = dict(param=A + o, grad=2 * A + o, exp_avg=3 * A + o, exp_avg_sq=4 * A + o, count=10, lr_scale=1.0, weight_decay=0.0)
         if bits == 8:
-            base |= dict(exp_avg_scale=A, exp_avg_sq_scale=A)
-        for k, v in (base | over).items():
-            setattr(rows[i], k, v)
+            base |= dict(exp_avg_scale=5 * A + o, exp_avg_sq_scale=6 * A + o)
+        rows += ops._TENSOR.pack(*[(base | over).get(f) or 0 for f in TENSOR_FIELDS])
     h = ctypes.c_void_p()
     rc = L.mscclAmdAdamWCreate(ctypes.byref(h) if plan else None, rows, n, paramType, gradType, bits, step, device, nbytes, None)
     assert not h
@@ -63,8 +67,11 @@ def adamw_create(tensor=None, n=1, paramType=F32, gradType=F32, bits=32, step=A,
     dict(tensor=dict(param=None)), dict(tensor=dict(grad=None)), dict(tensor=dict(exp_avg=None)),
     dict(tensor=dict(exp_avg_sq=None)), dict(bits=8, tensor=dict(exp_avg_scale=None)),
     dict(bits=8, tensor=dict(exp_avg_sq_scale=None)), dict(tensor=dict(exp_avg_scale=A)),
-    dict(tensor=dict(master=A)),                                    # a copy of 32-bit weights
-    dict(n=2, paramType=BF16, tensor=dict(master=A), second=dict()),  # only some have copies
+    dict(tensor=dict(master=9 * A)),                                    # a copy of 32-bit weights
+    dict(n=2, paramType=BF16, tensor=dict(master=9 * A), second=dict()),  # only some have copies
+    dict(n=2, second=dict(param=A)), dict(n=2, second=dict(exp_avg=3 * A + 36)),   # a tensor twice, one in another's end
+    dict(tensor=dict(exp_avg=A + 16)), dict(tensor=dict(grad=A + 20)), dict(tensor=dict(grad=7 * A)),
+    dict(bits=8, tensor=dict(exp_avg_sq_scale=5 * A)), dict(n=2, second=dict(grad=4 * A - 4)),
     dict(tensor=dict(param=A + 2)), dict(gradType=F16, tensor=dict(grad=A + 1)), dict(tensor=dict(exp_avg=A + 1)),
     dict(paramType=F16, tensor=dict(master=A + 2)), dict(bits=8, tensor=dict(exp_avg_scale=A + 2)),
     dict(tensor=dict(weight_decay=float("nan"))), dict(tensor=dict(lr_scale=float("inf"))),
@@ -93,7 +100,7 @@ def router(**kw):
 
 
 BAD_ROUTERS = [dict(type=I32), dict(type=M.FLOAT64), dict(score=2), dict(score=-1), dict(experts=0), dict(experts=1025),
-               dict(top_k=0), dict(top_k=9), dict(tokens=(1 << 30) + 1), dict(logit_stride=7), dict(logit_stride=1 << 40),
+               dict(top_k=0), dict(top_k=9), dict(tokens=(1 << 30) + 1), dict(tokens=1 << 30, top_k=1024, experts=1024), dict(logit_stride=7), dict(logit_stride=1 << 40),
                dict(logits=None), dict(logits=A + 2), dict(type=BF16, logits=A + 1)]
 
 
@@ -184,3 +191,26 @@ def test_router_struct_is_the_headers():
     raw = ops._ROUTER.pack(*values)
     r = Router.from_buffer_copy(raw.ljust(ctypes.sizeof(Router), b"\0"))
     assert [getattr(r, f) for f in FIELDS] == values
+
+
+def test_packed_structs_have_the_headers_sizes(tmp_path):
+    """Sizes and offsets of the packed argument structs as the C compiler sees them."""
+    import os
+    import shutil
+    import subprocess
+    if not shutil.which("gcc"):
+        pytest.skip("gcc missing")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src, exe = tmp_path / "s.c", str(tmp_path / "s")
+    src.write_text("""#include <stdio.h>
+#include "msccl_amd_ops.h"
+int main(void) {
+  printf("%zu %zu %zu %zu %zu\\n", sizeof(mscclAmdAdamWTensor_t), offsetof(mscclAmdAdamWTensor_t, lrScale),
+         offsetof(mscclAmdRouter_t, score), offsetof(mscclAmdRouter_t, topK), offsetof(mscclAmdAdamWTensor_t, count));
+  return 0;
+}
+""")
+    subprocess.run(["gcc", "-Wall", "-Werror", "-I" + os.path.join(root, "include"), "-I/opt/rocm/include",
+                    "-D__HIP_PLATFORM_AMD__", str(src), "-o", exe], check=True, capture_output=True, text=True)
+    got = [int(x) for x in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [ops._TENSOR.size, ops._TENSOR.size - 8, ops._ROUTER.size - 4, 56, 56]
