@@ -245,6 +245,26 @@ __device__ __forceinline__ float sumOver(float x) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
   }));
 }
+// the sum over the wave's lanes whose numbers are the same but for multiples of L (from far to near: what
+// a row rotation by 8, 4, 2 or 1 brings is the lane's partner, as all lanes twice as far apart hold the same)
+template <int L>
+__device__ __forceinline__ float sumAcross(float x) {
+  const auto f = [](uint32_t y) { return __builtin_bit_cast(float, y); };
+  const auto u = [](float y) { return __builtin_bit_cast(uint32_t, y); };
+  if constexpr (L <= 32) {
+    const auto y = __builtin_amdgcn_permlane32_swap(u(x), u(x), false, false);
+    x = f(y[0]) + f(y[1]);
+  }
+  if constexpr (L <= 16) {
+    const auto y = __builtin_amdgcn_permlane16_swap(u(x), u(x), false, false);
+    x = f(y[0]) + f(y[1]);
+  }
+  if constexpr (L <= 8) x += f(dpp<0x128>(u(x)));
+  if constexpr (L <= 4) x += f(dpp<0x124>(u(x)));
+  if constexpr (L <= 2) x += f(dpp<0x122>(u(x)));
+  if constexpr (L <= 1) x += f(dpp<0x121>(u(x)));
+  return x;
+}
 // a wave's sum of 64-bit values: the halves exchanged alike
 __device__ __forceinline__ double waveSum(double x) {
   const auto add = [](double a, uint32_t hi, uint32_t lo) { return a + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };

@@ -223,10 +223,7 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
       const Columns& c = j ? c1 : c0;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        if (half) {
-#pragma unroll
-          for (int d = 32; d >= LPR; d >>= 1) acc[j][i] += __shfl_xor(acc[j][i], d);
-        }
+        if (half) acc[j][i] = sumAcross<LPR>(acc[j][i]);
         if ((threadIdx.x & 63) < LPR && wave / (waves / 2) == half && c.has(i)) {
           float* s = &sums[wave % (waves / 2)][c.base + i];
           *s = half ? acc[j][i] : *s + acc[j][i];
@@ -403,7 +400,9 @@ static int lanesPerRow(int experts) {
 int balanceBlocks(int64_t tokens, int experts) {
   const int64_t rowsPer = kStatsThreads / lanesPerRow(experts);
   const int64_t passes = (tokens + rowsPer - 1) / rowsPer;
-  if (passes <= 1) return 1;
+  // One workgroup writes the results itself: 4 passes 8.6 us against 12.9 with the second launch enqueued
+  // one by one and 6.4 against 7.0 in a graph (64 experts), 8 passes 8.9 against 13 and 9.1 against 7.3.
+  if (passes <= 4) return 1;
   return (int)(passes < kStatsBlocks ? passes : kStatsBlocks);
 }
 

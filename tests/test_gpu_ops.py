@@ -282,6 +282,44 @@ def test_adamw_many_tensors(count, size, bits):
     assert int(k.step) == 1
 
 
+@pytest.mark.parametrize("chunks", [31, 32, 33, 500, 2100])
+def test_adamw_on_both_sides_of_one_launch(chunks):
+    for bits in (32, 8):
+        k = Model([2048 * chunks - 5], BF16, BF16, False, bits)
+        for t in range(1, 4):
+            want = k.want(1e-2, (0.9, 0.999), 1e-8)
+            k.plan.step(1e-2)
+            k.check(want, t)
+
+
+def test_offsets_past_32_bits():
+    """4.3 billion elements in one tensor: what lies behind the 2^32nd is stepped and summed like the rest."""
+    n, tail = (1 << 32) + 5003, 5000
+    grad = torch.zeros(n, dtype=BF16, device="cuda")
+    param = torch.ones(n, dtype=BF16, device="cuda")
+    m, v, ms, vs = ops.adamw_state(param, bits=8)
+    grad[-tail:] = torch.randn(tail, generator=gen(1), device="cuda").to(BF16)
+    grad[:3] = 2.0
+    total = ops.SquareSum([grad])()
+    want = float(grad[-tail:].double().square().sum()) + 12.0
+    assert abs(float(total) - want) <= want * n * 2.0 ** -52
+    small = Model([tail], BF16, BF16, False, 32, decay=0.0)
+    small.p[0].copy_(param[-tail:])
+    small.g[0].copy_(grad[-tail:])
+    step = torch.zeros(1, dtype=torch.int64, device="cuda")
+    ops.AdamW([param], [grad], [m], [v], step, exp_avg_scales=[ms], exp_avg_sq_scales=[vs]).step(1e-2)
+    small.plan.step(1e-2)
+    assert torch.equal(param[-tail:], small.p[0]) and int(step) == 1
+    assert bool((param[:3] < 1).all()) and bool((param[3:-tail] == 1).all())
+    first = (n - tail) // 256   # the first run that the tail reaches
+    got = ops.dequantize_state(m[first * 256:], ms[first:])[n - tail - first * 256:].double()
+    exact = small.g[0].double() * 0.1
+    # half a step of e4m3 (2^-4, or 2^-10 of the scale, itself the run's largest / 448) and its 6 roundings
+    near = ms[first:].double().repeat_interleave(256)[n - tail - first * 256:][:tail]
+    assert bool(((got - exact).abs() <= (2.0 ** -4 * exact.abs()).maximum(2.0 ** -10 * near) * (1 + 1e-5)).all())
+    assert int((ms != 0).sum()) <= tail // 256 + 3
+
+
 def test_adamw_large_tensor_and_step_count():
     k = Model([5_000_011], BF16, BF16, True, 32, t0=123_456)
     want = k.want(1e-3, (0.9, 0.999), 1e-8)
