@@ -82,7 +82,10 @@ size_t mscclAmdAdamWBytes(size_t n);
  * With states in 8 bits expAvg holds e4m3 codes (1 sign, 4 exponent, 3 fraction bits, largest 448) of
  * m / scale, and expAvgSq of sqrt(v) / scale, scale = the run's largest magnitude / 448; a second
  * moment above zero never gets the zero code (its step would be m / eps).  Codes and scales of zero
- * are the state before the first step.  A run that holds an infinity or NaN reads back as NaN. */
+ * are the state before the first step.  A run that holds an infinity or NaN reads back as NaN.
+ * Codes are rounded to nearest: one step must move sqrt(v) by half a code's step, 3.3 to 6.3 %, to
+ * change an element's code; slower changes show in the run's scale alone (beta2 0.95 follows gradients
+ * of 1.5 to 1.9 times the root of v, 0.999 of 8 to 11 times). */
 ncclResult_t mscclAmdAdamWCreate(mscclAmdAdamW_t* plan, const mscclAmdAdamWTensor_t* tensors, size_t n,
                                  ncclDataType_t paramType, ncclDataType_t gradType, int stateBits, int64_t* step,
                                  void* device, size_t deviceBytes, hipStream_t stream);
