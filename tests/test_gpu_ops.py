@@ -789,6 +789,35 @@ def test_balance_refuses():
         ops.balance_backward(logits, counts, 0)
 
 
+def test_calls_from_another_current_device(monkeypatch):
+    """The way round by the tensors' own device (taken once here, as if another were current)."""
+    x = torch.randn(1000, generator=gen(1), device="cuda")
+    logits, ind, valid = router(50, 12, 3, F32, True)
+    a, b = Model([300], seed=2), Model([300], seed=2)
+    plan = ops.SquareSum([x])
+    total = plan()
+    counts, probs = ops.balance_stats(logits, ind, valid=valid)
+    loss, grad = ops.balance_loss(counts, probs, 3), ops.balance_backward(logits, counts, 3, valid=valid)
+    b.plan.step(1e-2)
+    once = []
+
+    def elsewhere(device):
+        once.append(device)
+        return len(once) % 2 == 1
+
+    def check(call, *want):
+        once.clear()
+        got = call()
+        assert len(once) >= 1 and all(torch.equal(g, w) for g, w in zip(got, want))
+    monkeypatch.setattr(ops, "_elsewhere", elsewhere)
+    check(lambda: [plan()], total)
+    check(lambda: ops.balance_stats(logits, ind, valid=valid), counts, probs)
+    check(lambda: [ops.balance_loss(counts, probs, 3)], loss)
+    check(lambda: [ops.balance_backward(logits, counts, 3, valid=valid)], grad)
+    check(lambda: a.plan.step(1e-2) or [])
+    assert a.same(b.copy())
+
+
 # ---- a run of them, beside the collectives -----------------------------------------------------------
 
 @pytest.mark.parametrize("bits", [32, 8])
@@ -799,6 +828,51 @@ def test_a_sharded_training_step(bits):
     comms = M.Comm.init_all([0, 0])
     try:
         run_sharded(comms, bits)
+    finally:
+        torch.cuda.synchronize()
+        for c in comms:
+            c.destroy()
+
+
+def test_a_sharded_step_in_a_graph():
+    """Captured once and replayed, with gradients that change, against the same steps one by one."""
+    import msccl_amd as M
+    n, block = 2, 6400
+
+    def make(comms):
+        params = [(torch.randn(n * block, generator=gen(1), device="cuda") * 0.1).to(BF16) for _ in range(n)]
+        grads = [torch.zeros(n * block, dtype=BF16, device="cuda") for _ in range(n)]
+        shards = [torch.zeros(block, dtype=BF16, device="cuda") for _ in range(n)]
+        plans, sums, keep = [], [], []
+        for r in range(n):
+            p = params[r][r * block:(r + 1) * block]
+            w, st, step = p.float(), ops.adamw_state(p, 8), torch.zeros(1, dtype=torch.int64, device="cuda")
+            plans.append(ops.AdamW([p], [shards[r]], [st[0]], [st[1]], step, masters=[w], exp_avg_scales=[st[2]],
+                                   exp_avg_sq_scales=[st[3]], weight_decay=0.1))
+            sums.append(ops.SquareSum([shards[r]]))
+            keep += [w, *st, step]
+        return params, grads, shards, plans, sums, keep
+    comms = M.Comm.init_all([0] * n)
+    try:
+        a, b = make(comms), make(comms)
+        lr = torch.full((1,), 1e-2, device="cuda")
+        ops.sharded_step(comms, a[1], a[2], a[0], a[3], a[4], lr=1e-2, max_norm=1.0)   # gradients of zero
+        ops.sharded_step(comms, b[1], b[2], b[0], b[3], b[4], lr=1e-2, max_norm=1.0)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            totals = ops.sharded_step(comms, a[1], a[2], a[0], a[3], a[4], lr=[lr] * n, max_norm=1.0)
+        for t in range(1, 5):
+            lr.fill_(1e-2 / t)
+            for r in range(n):
+                a[1][r].copy_(torch.randn(n * block, generator=gen(10 * t + r), device="cuda"))
+                b[1][r].copy_(a[1][r])
+            graph.replay()
+            eager = ops.sharded_step(comms, b[1], b[2], b[0], b[3], b[4], lr=[lr] * n, max_norm=1.0)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(totals, eager))
+            assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a[0] + a[5], b[0] + b[5]))
+            assert int(a[5][-1]) == t + 1
     finally:
         torch.cuda.synchronize()
         for c in comms:
