@@ -122,7 +122,6 @@ __device__ __forceinline__ OPS_GLOBAL T* inGlobal(T* p) { return (OPS_GLOBAL T*)
 template <class T>
 __device__ __forceinline__ T scalarLoad(const T* p) { return *(const OPS_CONST T*)p; }
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 // N contiguous elements.  The vector types carry their element's alignment only: gfx950 loads and

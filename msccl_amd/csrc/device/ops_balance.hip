@@ -11,7 +11,7 @@
 // atomics (in LDS) give the same result in any order.  The statistics' workgroups are large and
 // few, one a CU, so that there are few partial sums to add (256; with 512 the second launch takes 1 us
 // longer than the first gains); the row after the one that is worked on is always on its way.
-// 131072 tokens of 256 experts in bfloat16: statistics 16.9 us (68 MiB; reading and adding alone take 12.4)
+// 131072 tokens of 256 experts in bfloat16: statistics 17 to 18 us (68 MiB; reading and adding alone take 12.4)
 // and 3.4 for the second launch, gradient 23.4 us (128 MiB, 5.7 TB/s).
 #include "ops.h"
 
