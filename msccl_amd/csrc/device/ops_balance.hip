@@ -51,16 +51,17 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
 #pragma unroll
       for (int i = 0; i < 8; i++) top = larger(x[j][i], top);
     top = maxOver<LPR>(top);
-    if (__builtin_expect(__ballot(!(fabsf(top) < 0x1p126f)) != 0, 0)) {
-      // Masked with the lowest value, infinite or nothing there: the difference itself.  A row of -inf alone
-      // has no scores; its sum stays 0.
+    if (__builtin_expect(__ballot(!(fabsf(top) < 0x1p20f)) != 0, 0)) {
+      // Large, masked with a low value throughout, infinite or nothing there: the difference itself.  A row of
+      // -inf alone has no scores; its sum stays 0.
       const float from = top == -__builtin_inff() ? 0.f : top;
 #pragma unroll
       for (int j = 0; j < VPL; j++)
 #pragma unroll
         for (int i = 0; i < 8; i++) x[j][i] = exp2Of((x[j][i] - from) * kLog2e);
     } else {
-      // One FMA: the rounding of top log2(e) is the same factor on every score of the row.
+      // One FMA: the rounding of top log2(e), at most 2^-4 here, is the same factor of 0.957 to 1.045 on every
+      // score of the row (without the bound above it would grow with top until the scores are inf or 0).
       const float from = -top * kLog2e;
 #pragma unroll
       for (int j = 0; j < VPL; j++)
@@ -75,7 +76,7 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
   return sum;
 }
 
-// One over the row's sum; 0 for a row without scores.  A softmax's is 1 to 1024, where the hardware's
+// One over the row's sum; 0 for a row without scores.  A softmax's is 0.95 to 1071, where the hardware's
 // reciprocal is within one unit; a sum of sigmoids may be as small as a 32-bit value gets.
 template <bool SIG>
 __device__ __forceinline__ float inverse(float z) {
