@@ -364,20 +364,35 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
     if (valid) {
       const float mine = scores<LPR, VPL, SIG, SIG>(x, slope);
       float dot = 0.f;
+      if constexpr (SIG) {
+        // A row's scores may all be small: the probabilities first, so that their products with the weights
+        // are of the weights' size and neither lose their digits nor pass 32 bits.
+        const float inv = inverse<SIG>(sumOver<LPR>(mine));
 #pragma unroll
-      for (int j = 0; j < VPL; j++)
+        for (int j = 0; j < VPL; j++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) dot = fmaf(x[j][i], w[j][i], dot);
-      const float inv = inverse<SIG>(sumOver<LPR>(mine));
-      // p (w - sum of w p) = s (w / z - (sum of w s) / z^2)
-      dot = sumOver<LPR>(dot) * inv * inv;
+          for (int i = 0; i < 8; i++) {
+            x[j][i] *= inv;
+            dot = fmaf(x[j][i], w[j][i], dot);
+          }
+        dot = sumOver<LPR>(dot);
 #pragma unroll
-      for (int j = 0; j < VPL; j++)
+        for (int j = 0; j < VPL; j++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          x[j][i] *= fmaf(w[j][i], inv, -dot);
-          if constexpr (SIG) x[j][i] *= slope[j][i];
-        }
+          for (int i = 0; i < 8; i++) x[j][i] *= (w[j][i] - dot) * slope[j][i];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VPL; j++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) dot = fmaf(x[j][i], w[j][i], dot);
+        const float inv = inverse<SIG>(sumOver<LPR>(mine));
+        // p (w - sum of w p) = s (w / z - (sum of w s) / z^2): both sums over the row at once
+        dot = sumOver<LPR>(dot) * inv * inv;
+#pragma unroll
+        for (int j = 0; j < VPL; j++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[j][i] *= fmaf(w[j][i], inv, -dot);
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < VPL; j++) x[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};

@@ -110,3 +110,25 @@ def test_softmax_rows_masked_throughout_weigh_alike():
         x = torch.full((64, 8), low, device="cuda")
         counts, probs = ops.balance_stats(x, torch.zeros(64, 2, dtype=torch.int64, device="cuda"))
         assert probs.tolist() == [8.0] * 8, low
+
+
+@pytest.mark.parametrize("experts", EXPERTS)
+@pytest.mark.parametrize("up", [1e-30, 1e-6, 1.0, 1e14, 1e25])
+def test_sigmoid_gradient_where_all_scores_are_small(experts, up):
+    """The mean of the weights over a row is of the weights' size, however small the scores are: it neither
+    loses its digits in 32 bits nor passes their range."""
+    x = -73.0 - 12.0 * torch.rand(64, experts, generator=gen(4), device="cuda")
+    counts = torch.randint(1, 100_000, (experts + 1,), generator=gen(5), device="cuda")
+    counts[experts] = 1_000_000
+    k = min(2, experts)
+    got = ops.balance_backward(x, counts, k, 0.01, grad_output=torch.full((1,), up, device="cuda"), score="sigmoid")
+    p = definition(x, "sigmoid")[0]
+    scale = 0.01 * experts / (k * 1e12) * up
+    w = (counts[:experts].double() - 1e6 * k / experts) * scale
+    mean = (p * w).sum(1, keepdim=True)
+    d = p * (w - mean)
+    # a score: its exponential's argument 1.3 |x|, and 8; a probability that of the sum's terms too, 15
+    # additions, the quotient 2; the weights 3; the mean's terms as many again, and 17 additions
+    err = 2.6 * x.double().abs() + 33
+    bound = U * p * ((err + 10) * (w - mean).abs() + (p * w.abs()).sum(1, keepdim=True) * (err + 20)) + 2.0 ** -140
+    close(got, d, bound, "gradient")
