@@ -26,14 +26,46 @@ __device__ __forceinline__ float exp2Of(float t) { return __builtin_amdgcn_exp2f
 // max(a, b), or b where a is not a number; one instruction (the library's makes its operands quiet first)
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
 
-// The row's unnormalised scores in place of its logits: e^(x - max) or sigmoid(x) (0 outside the row).
-// Returns the lane's part of their sum.  SLOPE: also 1 - sigmoid(x), which 1 - s would round away near 1.
+// e^(x - top) of a row, by the difference itself: right for any finite top.  A row of -inf alone has no scores.
+template <int VPL>
+__device__ __forceinline__ void differences(f32x8 (&x)[VPL], float top) {
+  const float from = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+  for (int j = 0; j < VPL; j++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[j][i] = exp2Of((x[j][i] - from) * kLog2e);
+}
+
+template <int LPR, int VPL>
+__device__ __forceinline__ float largest(const f32x8 (&x)[VPL]) {
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < VPL; j++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = larger(x[j][i], top);
+  return maxOver<LPR>(top);
+}
+
+template <int LPR, int VPL>
+__device__ __forceinline__ float total(const f32x8 (&x)[VPL]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < VPL; j++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += x[j][i];
+  return sumOver<LPR>(sum);
+}
+
+// The row's unnormalised scores in place of its logits: e^(x - max) or sigmoid(x) (0 outside the row), or
+// what is in proportion to them.  Returns their sum.  SLOPE: also 1 - sigmoid(x), which 1 - s would round
+// away near 1.
 template <int LPR, int VPL, bool SIG, bool SLOPE>
 __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
-  float sum = 0.f;
   if constexpr (SIG) {
+    f32x8 logit[VPL];
 #pragma unroll
-    for (int j = 0; j < VPL; j++)
+    for (int j = 0; j < VPL; j++) {
+      logit[j] = x[j];
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         // e = e^-|x|: 1 / (1 + e), or e / (1 + e) left of zero (the reciprocal of 1 to 2: within one unit)
@@ -42,23 +74,27 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
         const bool right = x[j][i] >= 0.f;
         if constexpr (SLOPE) slope[j][i] = right ? er : r;
         x[j][i] = right ? r : er;
-        sum += x[j][i];
       }
+    }
+    float z = total<LPR, VPL>(x);
+    const bool far = z < 0x1p-25f;
+    if (__builtin_expect(__ballot(far) != 0, 0)) {
+      // Every logit is below -17: 1 + e^x is one, and e^(x - max) in proportion to the scores, which leave 32
+      // bits from -87 on.  Above that a score that the exponential flushes is less than 2^-101 of the sum.
+      const float top = largest<LPR, VPL>(logit);
+      if (far) {
+        differences<VPL>(logit, top);
+#pragma unroll
+        for (int j = 0; j < VPL; j++) x[j] = logit[j];
+        z = total<LPR, VPL>(x);
+      }
+    }
+    return z;
   } else {
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int j = 0; j < VPL; j++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) top = larger(x[j][i], top);
-    top = maxOver<LPR>(top);
+    const float top = largest<LPR, VPL>(x);
     if (__builtin_expect(__ballot(!(fabsf(top) < 0x1p20f)) != 0, 0)) {
-      // Large, masked with a low value throughout, infinite or nothing there: the difference itself.  A row of
-      // -inf alone has no scores; its sum stays 0.
-      const float from = top == -__builtin_inff() ? 0.f : top;
-#pragma unroll
-      for (int j = 0; j < VPL; j++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[j][i] = exp2Of((x[j][i] - from) * kLog2e);
+      // Large, masked with a low value throughout, infinite or nothing there.
+      differences<VPL>(x, top);
     } else {
       // One FMA: the rounding of top log2(e), at most 2^-4 here, is the same factor of 0.957 to 1.045 on every
       // score of the row (without the bound above it would grow with top until the scores are inf or 0).
@@ -68,16 +104,12 @@ __device__ __forceinline__ float scores(f32x8 (&x)[VPL], f32x8* slope) {
 #pragma unroll
         for (int i = 0; i < 8; i++) x[j][i] = exp2Of(fmaf(x[j][i], kLog2e, from));
     }
-#pragma unroll
-    for (int j = 0; j < VPL; j++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) sum += x[j][i];
+    return total<LPR, VPL>(x);
   }
-  return sum;
 }
 
 // One over the row's sum; 0 for a row without scores.  A softmax's is 0.95 to 1071, where the hardware's
-// reciprocal is within one unit; a sum of sigmoids may be as small as a 32-bit value gets.
+// reciprocal is within one unit; a sum of sigmoids 2^-25 to 1024.
 template <bool SIG>
 __device__ __forceinline__ float inverse(float z) {
   if constexpr (SIG) return z == 0.f ? 0.f : 1.f / z;
@@ -201,8 +233,7 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
     }
     if (!now) continue;   // (whatever the row holds)
     here++;
-    const float z = sumOver<LPR>(scores<LPR, VPL, SIG, false>(x, nullptr));
-    const float inv = inverse<SIG>(z);
+    const float inv = inverse<SIG>(scores<LPR, VPL, SIG, false>(x, nullptr));
 #pragma unroll
     for (int j = 0; j < VPL; j++)
 #pragma unroll
@@ -362,12 +393,11 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
     }
     if (ACC && !valid) continue;
     if (valid) {
-      const float mine = scores<LPR, VPL, SIG, SIG>(x, slope);
+      const float inv = inverse<SIG>(scores<LPR, VPL, SIG, SIG>(x, slope));
       float dot = 0.f;
       if constexpr (SIG) {
-        // A row's scores may all be small: the probabilities first, so that their products with the weights
-        // are of the weights' size and neither lose their digits nor pass 32 bits.
-        const float inv = inverse<SIG>(sumOver<LPR>(mine));
+        // A row's scores may be small: the probabilities first, so that their products with the weights are of
+        // the weights' size and neither lose their digits nor pass 32 bits.
 #pragma unroll
         for (int j = 0; j < VPL; j++)
 #pragma unroll
@@ -385,8 +415,7 @@ __global__ void __launch_bounds__(kOpsThreads) balanceBackwardKernel(BalanceArgs
         for (int j = 0; j < VPL; j++)
 #pragma unroll
           for (int i = 0; i < 8; i++) dot = fmaf(x[j][i], w[j][i], dot);
-        const float inv = inverse<SIG>(sumOver<LPR>(mine));
-        // p (w - sum of w p) = s (w / z - (sum of w s) / z^2): both sums over the row at once
+        // p (w - sum of w p) = s (w / z - (sum of w s) / z^2): the row's two sums do not wait for one another
         dot = sumOver<LPR>(dot) * inv * inv;
 #pragma unroll
         for (int j = 0; j < VPL; j++)

@@ -37,9 +37,10 @@ def definition(x, score):
     err = 2.3 * d + 43
     if score == "sigmoid":
         # near zero instead: the exponential's argument 1.3 |x|, its own 2, the sum, the reciprocal and the
-        # product 4; the sum's terms the same, weighing as p does; 15 additions, quotient and product 2
+        # product 4; the sum's terms the same, weighing as p does; 15 additions, quotient and product 2.
+        # (a sum of 1024 scores below e^-26 is below 2^-25: from there on the differences count again)
         far = x.abs().clamp(max=150.0)
-        err = torch.where(x.amax(1, keepdim=True) > -18, 1.3 * far + (p * 1.3 * far).sum(1, keepdim=True) + 30, err)
+        err = torch.where(x.amax(1, keepdim=True) > -26, 1.3 * far + (p * 1.3 * far).sum(1, keepdim=True) + 30, err)
     return p, torch.special.expit(-x), err
 
 
@@ -132,3 +133,32 @@ def test_sigmoid_gradient_where_all_scores_are_small(experts, up):
     err = 2.6 * x.double().abs() + 33
     bound = U * p * ((err + 10) * (w - mean).abs() + (p * w.abs()).sum(1, keepdim=True) * (err + 20)) + 2.0 ** -140
     close(got, d, bound, "gradient")
+
+
+LOW = [-15.0, -17.0, -17.5, -18.0, -25.0, -60.0, -70.0, -85.0, -87.0, -88.0, -95.0, -103.0, -150.0, -1e3, -60000.0, -1e10, -1e30, -3.4e38]
+
+
+@pytest.mark.parametrize("experts", EXPERTS)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_sigmoid_rows_far_below_zero(dtype, experts):
+    """Their scores leave 32 bits, their probabilities do not."""
+    g = gen(6)
+    rows = [rows_at(LOW, experts, dtype)]
+    for v in LOW:   # a few units apart from each other, as scores of one row are
+        rows.append((v - 6.0 * torch.rand(3, experts, generator=g, device="cuda", dtype=torch.float64)).clamp(min=float(torch.finfo(dtype).min)).to(dtype))
+    check_rows(torch.cat(rows), "sigmoid")
+    for r in rows[1:]:
+        check_rows(r, "sigmoid")
+
+
+def test_sigmoid_rows_between_infinities():
+    """A row of -inf alone has nothing; one score among them has everything; +inf counts as one does."""
+    inf = float("inf")
+    x = torch.tensor([[-inf] * 4, [-inf, -200.0, -inf, -inf], [-90.0, -inf, -90.0, -inf], [inf, -300.0, -inf, inf]], device="cuda")
+    index = torch.zeros(4, 1, dtype=torch.int32, device="cuda")
+    for r, want in enumerate([[0, 0, 0, 0], [0, 1, 0, 0], [0.5, 0, 0.5, 0], [0.5, 0, 0, 0.5]]):
+        assert ops.balance_stats(x[r:r + 1], index[r:r + 1], score="sigmoid")[1].tolist() == want
+    got = ops.balance_backward(x, torch.tensor([5, 1, 1, 1, 4], device="cuda"), 1, score="sigmoid")
+    assert bool(torch.isfinite(got).all()) and float(got[:2].abs().max()) == 0 and float(got[3].abs().max()) == 0
+    # p (w - mean) of weights 20 / 16 and 1 / 4 on halves
+    assert got[2].tolist() == [0.25, 0, -0.25, 0]
