@@ -135,7 +135,7 @@ size_t mscclAmdBalanceWorkspace(size_t tokens, size_t experts);
 
 /* counts[0..experts): the slots of valid tokens that chose the expert; counts[experts]: the valid
  * tokens.  probs[0..experts): the sum over valid tokens of p, of any finite logits (a p below 2^-100 may
- * be taken as zero).  A row whose logits are all -inf adds nothing to probs; one with a NaN logit adds
+ * be taken as zero), added up in 64 bits and rounded once.  A row whose logits are all -inf adds nothing to probs; one with a NaN logit adds
  * NaN, and under softmax one with a logit of +inf.
  * Summed over the ranks (ncclAllReduce in ncclInt64 and ncclFloat32) they are the whole batch's. */
 ncclResult_t mscclAmdBalanceStats(const mscclAmdRouter_t* router, int64_t* counts, float* probs, void* workspace,

@@ -78,8 +78,8 @@ struct BalanceArgs {
   // statistics
   int64_t* counts;
   float* probs;
+  double* probPart;      // [grid][experts], 4-byte aligned
   uint32_t* countPart;   // [grid][experts + 1]
-  float* probPart;       // [grid][experts]
   // gradient
   const int64_t* countsIn;
   const float* gradLoss;
@@ -244,31 +244,36 @@ __device__ __forceinline__ float sumOver(float x) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
   }));
 }
-// the sum over the wave's lanes whose numbers are the same but for multiples of L (from far to near: what
-// a row rotation by 8, 4, 2 or 1 brings is the lane's partner, as all lanes twice as far apart hold the same)
+// the sum of 64-bit values over the wave's lanes whose numbers are the same but for multiples of L, the
+// halves exchanged alike (from far to near: what a row rotation by 8, 4, 2 or 1 brings is the lane's partner,
+// as all lanes twice as far apart hold the same)
+__device__ __forceinline__ double fromHalves(uint32_t hi, uint32_t lo) {
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 template <int L>
-__device__ __forceinline__ float sumAcross(float x) {
-  const auto f = [](uint32_t y) { return __builtin_bit_cast(float, y); };
-  const auto u = [](float y) { return __builtin_bit_cast(uint32_t, y); };
+__device__ __forceinline__ double sumAcross(double x) {
+  const auto hi = [](double y) { return (uint32_t)(__builtin_bit_cast(uint64_t, y) >> 32); };
+  const auto lo = [](double y) { return (uint32_t)__builtin_bit_cast(uint64_t, y); };
   if constexpr (L <= 32) {
-    const auto y = __builtin_amdgcn_permlane32_swap(u(x), u(x), false, false);
-    x = f(y[0]) + f(y[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(hi(x), hi(x), false, false);
+    const auto l = __builtin_amdgcn_permlane32_swap(lo(x), lo(x), false, false);
+    x = fromHalves(h[0], l[0]) + fromHalves(h[1], l[1]);
   }
   if constexpr (L <= 16) {
-    const auto y = __builtin_amdgcn_permlane16_swap(u(x), u(x), false, false);
-    x = f(y[0]) + f(y[1]);
+    const auto h = __builtin_amdgcn_permlane16_swap(hi(x), hi(x), false, false);
+    const auto l = __builtin_amdgcn_permlane16_swap(lo(x), lo(x), false, false);
+    x = fromHalves(h[0], l[0]) + fromHalves(h[1], l[1]);
   }
-  if constexpr (L <= 8) x += f(dpp<0x128>(u(x)));
-  if constexpr (L <= 4) x += f(dpp<0x124>(u(x)));
-  if constexpr (L <= 2) x += f(dpp<0x122>(u(x)));
-  if constexpr (L <= 1) x += f(dpp<0x121>(u(x)));
+  if constexpr (L <= 8) x += fromHalves(dpp<0x128>(hi(x)), dpp<0x128>(lo(x)));
+  if constexpr (L <= 4) x += fromHalves(dpp<0x124>(hi(x)), dpp<0x124>(lo(x)));
+  if constexpr (L <= 2) x += fromHalves(dpp<0x122>(hi(x)), dpp<0x122>(lo(x)));
+  if constexpr (L <= 1) x += fromHalves(dpp<0x121>(hi(x)), dpp<0x121>(lo(x)));
   return x;
 }
 // a wave's sum of 64-bit values: the halves exchanged alike
 __device__ __forceinline__ double waveSum(double x) {
-  const auto add = [](double a, uint32_t hi, uint32_t lo) { return a + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };
 #define OPS_STEP(CTRL) do { const uint64_t b = __builtin_bit_cast(uint64_t, x); \
-    x = add(x, dpp<CTRL>((uint32_t)(b >> 32)), dpp<CTRL>((uint32_t)b)); } while (0)
+    x += fromHalves(dpp<CTRL>((uint32_t)(b >> 32)), dpp<CTRL>((uint32_t)b)); } while (0)
   OPS_STEP(0xB1);
   OPS_STEP(0x4E);
   OPS_STEP(0x141);

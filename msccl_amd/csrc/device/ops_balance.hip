@@ -7,7 +7,10 @@
 // the registers of the 1 to 64 lanes that share it, 8 or 16 logits each, so nothing is read twice and
 // the sums over a row are lane exchanges.  A lane's columns are the same in every row it takes: the
 // sums over rows stay in its registers too, then one exchange through LDS and one partial sum a
-// workgroup, which a second launch adds in a fixed order in 64 bits.  Counts are integers: their
+// workgroup, which a second launch adds in a fixed order.  They are in 64 bits throughout and rounded once:
+// a router that starts from zero weights has equal rows, whose roundings in 32 bits do not average out
+// (a 64-bit FMA issues as a 32-bit one does; with the conversions it costs 0.45 us of the long batch's 21.2).
+// Counts are integers: their
 // atomics (in LDS) give the same result in any order.  The statistics' workgroups are large and
 // few, one a CU, so that there are few partial sums to add (256; with 512 the second launch takes 1 us
 // longer than the first gains); the row after the one that is worked on is always on its way.
@@ -155,6 +158,7 @@ __device__ __forceinline__ f32x8 ownColumns(const V& raw, const Columns& c, floa
 }
 
 constexpr int kStatsThreads = 1024;
+typedef double Double4 __attribute__((aligned(4)));   // (the caller's scratch is at a 4-byte boundary)
 
 template <class T, int LPR, int VPL, bool SIG, bool IDX64>
 __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs a, int64_t rowsEach) {
@@ -164,7 +168,8 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
   constexpr int copies = width <= 128 ? waves : 1;   // few experts: every wave counts by itself
   __shared__ uint32_t hist[copies][width];
   __shared__ uint32_t tokens;
-  __shared__ float sums[waves / 2][width];
+  constexpr int rooms = width <= 512 ? waves / 2 : waves / 4;   // (32 KiB of sums at most)
+  __shared__ double sums[rooms][width];
   const int wave = threadIdx.x / 64;
   const int64_t begin = blockIdx.x * rowsEach;
   const int64_t first = begin < a.tokens ? begin : a.tokens;   // (the last workgroups may have none)
@@ -210,15 +215,11 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
         atomicAdd(&hist[copies == 1 ? 0 : wave][e[k]], 1u);
   }
 
-  // 64 rows at most are added up in 32 bits; those sums in 64
-  f32x8 acc[VPL];
-  double total[VPL][8];
+  double acc[VPL][8];
 #pragma unroll
-  for (int j = 0; j < VPL; j++) {
-    acc[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};
+  for (int j = 0; j < VPL; j++)
 #pragma unroll
-    for (int i = 0; i < 8; i++) total[j][i] = 0.0;
-  }
+    for (int i = 0; i < 8; i++) acc[j][i] = 0.0;
   uint32_t here = 0;
   for (int r = own; r < rows; r += rowsPer) {
     f32x8 x[VPL];
@@ -233,39 +234,30 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
     }
     if (!now) continue;   // (whatever the row holds)
     here++;
-    const float inv = inverse<SIG>(scores<LPR, VPL, SIG, false>(x, nullptr));
+    const double inv = inverse<SIG>(scores<LPR, VPL, SIG, false>(x, nullptr));
 #pragma unroll
     for (int j = 0; j < VPL; j++)
 #pragma unroll
-      for (int i = 0; i < 8; i++) acc[j][i] = fmaf(x[j][i], inv, acc[j][i]);
-    if (here % 64 == 0) {
-#pragma unroll
-      for (int j = 0; j < VPL; j++) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) total[j][i] += (double)acc[j][i];
-        acc[j] = (f32x8){0, 0, 0, 0, 0, 0, 0, 0};
-      }
-    }
-  }
-  if (here >= 64) {
-#pragma unroll
-    for (int j = 0; j < VPL; j++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) acc[j][i] = (float)(total[j][i] + (double)acc[j][i]);
+      for (int i = 0; i < 8; i++) acc[j][i] = fma((double)x[j][i], inv, acc[j][i]);
   }
   if (here && lane == 0) atomicAdd(&tokens, here);
-  // over the wave's rows, then over the waves: the upper half's on top of the lower half's
+  // over the wave's rows, then over the waves: some of them first, then the others on top
 #pragma unroll
-  for (int half = 1; half >= 0; half--) {
+  for (int j = 0; j < VPL; j++)
 #pragma unroll
-    for (int j = 0; j < VPL; j++) {
-      const Columns& c = j ? c1 : c0;
+    for (int i = 0; i < 8; i++) acc[j][i] = sumAcross<LPR>(acc[j][i]);
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        if (half) acc[j][i] = sumAcross<LPR>(acc[j][i]);
-        if ((threadIdx.x & 63) < LPR && wave / (waves / 2) == half && c.has(i)) {
-          float* s = &sums[wave % (waves / 2)][c.base + i];
-          *s = half ? acc[j][i] : *s + acc[j][i];
+  for (int turn = 0; turn < waves / rooms; turn++) {
+    if ((threadIdx.x & 63) < LPR && wave / rooms == turn) {
+#pragma unroll
+      for (int j = 0; j < VPL; j++) {
+        const Columns& c = j ? c1 : c0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          if (c.has(i)) {
+            double* s = &sums[wave % rooms][c.base + i];
+            *s = turn == 0 ? acc[j][i] : *s + acc[j][i];
+          }
         }
       }
     }
@@ -273,17 +265,17 @@ __global__ void __launch_bounds__(kStatsThreads) balanceStatsKernel(BalanceArgs 
   }
   const bool only = gridDim.x == 1;
   for (int e = threadIdx.x; e < a.experts; e += kStatsThreads) {
-    float s = sums[0][e];
+    double s = sums[0][e];
 #pragma unroll
-    for (int w = 1; w < waves / 2; w++) s += sums[w][e];
+    for (int w = 1; w < rooms; w++) s += sums[w][e];
     uint32_t n = hist[0][e];
 #pragma unroll
     for (int w = 1; w < copies; w++) n += hist[w][e];
     if (only) {
-      a.probs[e] = s;
+      a.probs[e] = (float)s;
       a.counts[e] = n;
     } else {
-      a.probPart[(size_t)blockIdx.x * a.experts + e] = s;
+      *(Double4*)(a.probPart + (size_t)blockIdx.x * a.experts + e) = s;
       a.countPart[(size_t)blockIdx.x * (a.experts + 1) + e] = n;
     }
   }
@@ -303,19 +295,19 @@ __global__ void __launch_bounds__(1024) balanceFinishKernel(BalanceArgs a, int b
   __shared__ int64_t cs[16][16];
   const int col = threadIdx.x % 16, slice = threadIdx.x / 16;
   const int e = blockIdx.x * 16 + col;
-  float p[each];
+  double p[each];
   uint32_t c[each];
 #pragma unroll
   for (int k = 0; k < each; k++) {
     const int b = k * 64 + slice;
-    p[k] = b < blocks && e < a.experts ? a.probPart[(size_t)b * a.experts + e] : 0.f;
+    p[k] = b < blocks && e < a.experts ? *(const Double4*)(a.probPart + (size_t)b * a.experts + e) : 0.0;
     c[k] = b < blocks && e <= a.experts ? a.countPart[(size_t)b * (a.experts + 1) + e] : 0;
   }
   double p0 = 0.0;
   int64_t c0 = 0;
 #pragma unroll
   for (int k = 0; k < each; k++) {
-    p0 += (double)p[k];
+    p0 += p[k];
     c0 += (int64_t)c[k];
   }
 #pragma unroll

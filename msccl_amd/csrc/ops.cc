@@ -346,7 +346,7 @@ static ncclResult_t checkRouter(const char* name, const mscclAmdRouter_t* r, boo
 size_t mscclAmdBalanceWorkspace(size_t tokens, size_t experts) {
   if (tokens > (size_t)1 << 30 || experts < 1 || experts > (size_t)kMaxExperts) return 0;
   const size_t blocks = (size_t)balanceBlocks((int64_t)tokens, (int)experts);
-  return blocks == 1 ? 0 : blocks * (2 * experts + 1) * 4;
+  return blocks == 1 ? 0 : blocks * (experts * 8 + (experts + 1) * 4);
 }
 
 ncclResult_t mscclAmdBalanceStats(const mscclAmdRouter_t* router, int64_t* counts, float* probs, void* workspace,
@@ -361,8 +361,8 @@ ncclResult_t mscclAmdBalanceStats(const mscclAmdRouter_t* router, int64_t* count
   const int blocks = balanceBlocks(a.tokens, a.experts);
   a.counts = counts;
   a.probs = probs;
-  a.probPart = (float*)workspace;
-  a.countPart = (uint32_t*)workspace + (size_t)blocks * a.experts;
+  a.probPart = (double*)workspace;
+  a.countPart = (uint32_t*)workspace + (size_t)blocks * a.experts * 2;
   if (launchBalanceStats(a, router->type, router->indexType == ncclInt64, router->score == mscclAmdSigmoid, blocks, stream)) {
     WARN("%s : launch failed", name);
     return ncclUnhandledCudaError;

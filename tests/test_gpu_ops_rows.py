@@ -162,3 +162,16 @@ def test_sigmoid_rows_between_infinities():
     assert bool(torch.isfinite(got).all()) and float(got[:2].abs().max()) == 0 and float(got[3].abs().max()) == 0
     # p (w - mean) of weights 20 / 16 and 1 / 4 on halves
     assert got[2].tolist() == [0.25, 0, -0.25, 0]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens,experts", [(1000, 3), (40_000, 7), (5000, 60), (131_072, 100), (999_999, 100), (100_000, 200), (65_536, 700)])
+def test_equal_rows_add_up(tokens, experts, score):
+    """A router whose weights are zero: every row the same, so that the roundings of a sum do not average out."""
+    x = torch.zeros(tokens, experts, dtype=BF16, device="cuda")
+    counts, probs = ops.balance_stats(x, torch.zeros(tokens, 1, dtype=torch.int32, device="cuda"), score=score)
+    want = tokens / experts
+    # one over the row's sum (exact here) is within 2 roundings, its product with the score 1; the sums are in
+    # 64 bits and rounded once
+    assert int(counts[experts]) == tokens and float((probs.double() - want).abs().max()) <= 4 * U * want * (1 + 1e-6)
+
