@@ -83,12 +83,23 @@ size_t mscclAmdAdamWBytes(size_t n);
  * m / scale, and expAvgSq of sqrt(v) / scale, scale = the run's largest magnitude / 448; a second
  * moment above zero never gets the zero code (its step would be m / eps).  Codes and scales of zero
  * are the state before the first step.  A run that holds an infinity or NaN reads back as NaN.
- * Codes are rounded to nearest: one step must move sqrt(v) by half a code's step, 3.3 to 6.3 %, to
- * change an element's code; slower changes show in the run's scale alone (beta2 0.95 follows gradients
- * of 1.5 to 1.9 times the root of v, 0.999 of 8 to 11 times). */
+ * Codes are rounded to nearest unless mscclAmdAdamWSetRounding says otherwise. */
 ncclResult_t mscclAmdAdamWCreate(mscclAmdAdamW_t* plan, const mscclAmdAdamWTensor_t* tensors, size_t n,
                                  ncclDataType_t paramType, ncclDataType_t gradType, int stateBits, int64_t* step,
                                  void* device, size_t deviceBytes, hipStream_t stream);
+
+typedef enum { mscclAmdNearest = 0, mscclAmdStochastic = 1 } mscclAmdRounding_t;
+
+/* How the steps enqueued from now on round states of 8 bits (a plan begins with mscclAmdNearest; no
+ * device call).  To follow averages over many steps they need mscclAmdStochastic: a code becomes one of
+ * the two next to its value, so that m and v (not its root) are right in the mean, step after step.  Which
+ * one follows from seed, step count and the element's place in the plan: the same inputs give the same
+ * bits again.  One element's root of v is then within about a sixth (beta2 0.999) of the 32-bit state's.
+ * mscclAmdNearest is exact to half a code's step (3.1 to 6.3 % of the value) within a step, and loses what
+ * changes by less in every step: a decay of the root of v by 1 - sqrt(beta2), 2.5 % at 0.95 and 0.05 % at
+ * 0.999, never lowers a code, and an element whose code stays follows its run's scale, so that second
+ * moments beside a growing one grow with it for good.  It suits beta2 up to 0.93. */
+ncclResult_t mscclAmdAdamWSetRounding(mscclAmdAdamW_t plan, mscclAmdRounding_t rounding, uint64_t seed);
 
 /* Other gradient buffers for all n tensors (host array of device addresses, read now), from `stream`'s
  * next step on. */

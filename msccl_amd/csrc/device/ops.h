@@ -41,6 +41,7 @@ struct AdamControl {
   double rate;       // lr / (1 - beta1^t)
   float invRoot;     // 1 / sqrt(1 - beta2^t)
   float coef;        // on the gradients
+  int64_t t;         // the step's number
   int skip;
   uint32_t arrived;  // workgroups of a one-launch step that have read the step count; 0 between steps
 };
@@ -64,6 +65,7 @@ struct AdamStepArgs {
   double maxNorm;
   int64_t* step;
   float b1, c1, b2, c2, eps;
+  uint64_t seed;     // of the states' rounding, where that is by chance
 };
 
 struct BalanceArgs {
@@ -92,7 +94,7 @@ struct BalanceArgs {
 int launchTableWrite(void* dst, const void* host, size_t bytes, void* stream);
 int launchGradWrite(AdamTensor* rows, const void* const* grads, size_t n, void* stream);
 int launchSquareSum(const TensorTable<SumTensor>& tab, int type, double* out, double* partials, int blocks, void* stream);
-int launchAdamW(const AdamStepArgs& a, int paramType, int gradType, bool master, int bits, void* stream);
+int launchAdamW(const AdamStepArgs& a, int paramType, int gradType, bool master, int bits, bool dice, void* stream);
 int balanceBlocks(int64_t tokens, int experts);   // workgroups of the statistics; one needs no scratch
 int launchBalanceStats(const BalanceArgs& a, int type, bool index64, bool sigmoid, int blocks, void* stream);
 int launchBalanceLoss(const int64_t* counts, const float* probs, int experts, double scale, float* loss, void* stream);

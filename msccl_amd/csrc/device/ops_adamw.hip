@@ -10,6 +10,9 @@
 // (134M: 350 us, twice 369).  Where 8-bit states stand beside 16-bit tensors alone it takes 8 neighbours,
 // 16 bytes of those (46M: 80 us, twice 4 82, once 4 89).  256 elements that share a scale are then one or
 // half a wave's.  That is 5.8 to 6.15 TB/s; loads that do not stream past the caches make it 5.3.
+// 8-bit states rounded by chance take 20 more instructions an element, hidden behind the loads where there are
+// 32-bit tensors (134M with a 32-bit copy: 348 -> 356 us; 46M 32-bit weights 120 -> 124), not where all are
+// narrow (46M bfloat16: 80 -> 95).
 #include "ops.h"
 
 namespace msccl {
@@ -79,6 +82,7 @@ __device__ __forceinline__ AdamControl adamwControl(const AdamStepArgs& a, int64
   r.rate = r.lr / (1.0 - p1);
   r.invRoot = (float)(1.0 / sqrt(1.0 - p2));
   r.coef = (float)c;
+  r.t = t;
   r.skip = !ok;
   r.arrived = 0;
   return r;
@@ -91,6 +95,7 @@ __global__ void adamwBeginKernel(AdamStepArgs a) {
   a.ctl->rate = r.rate;
   a.ctl->invRoot = r.invRoot;
   a.ctl->coef = r.coef;
+  a.ctl->t = r.t;
   a.ctl->skip = r.skip;
   if (!r.skip) *a.step = taken + 1;
 }
@@ -116,11 +121,50 @@ __device__ __forceinline__ typename VecOf<float, N>::F decode(typename BytesOf<N
   return x;
 }
 
-// Codes and scale of a run (256 / N lanes, N values each).  FLOOR: no value above zero gets code zero.
-// A rounding to 3 fraction bits is off by at most 2^-4 of the value; values under 2^-10 of the unit
-// (scale) become zero.  Where a value is not finite the scale is NaN, and the codes say nothing.
-template <int N, bool FLOOR>
-__device__ __forceinline__ typename BytesOf<N>::V encode(const typename VecOf<float, N>::F& x, float& scale) {
+// ---- rounding by chance -------------------------------------------------------------------------
+// A step moves an average by less than half a code's step, so that rounded to nearest it would never arrive.
+// Numbers that look random, the same again for the same seed, step and place: multiplications by odd
+// constants of linear congruential generators, with the high half folded onto the low one between them.
+
+// what a chunk's elements share
+__device__ __forceinline__ uint64_t diceOf(uint64_t seed, uint64_t t, uint32_t chunk) {
+  constexpr uint64_t a = 6364136223846793005ull, b = 0x9e3779b97f4a7c15ull;
+  uint64_t k = seed + t * b;
+  k = (k ^ k >> 32) * a;
+  k = ((k ^ k >> 29) + chunk) * b;
+  k = (k ^ k >> 32) * a;
+  return k ^ k >> 32;
+}
+
+// the lane's number for its elements from `first` of the chunk on, and the i-th element's
+__device__ __forceinline__ uint32_t diceAt(uint64_t key, uint32_t first) {
+  uint32_t x = (uint32_t)key + first * 0x9e3779b1u;
+  x = (x ^ x >> 16) * 747796405u;
+  x = ((x ^ x >> 15) + (uint32_t)(key >> 32)) * 2891336453u;
+  return x ^ x >> 16;
+}
+__device__ __forceinline__ uint32_t throwOf(uint32_t lane, int i) {
+  constexpr uint32_t odd[8] = {0x9e3779b1u, 0x7f4a7c15u, 0x2c9277b5u, 0xac564b05u, 0xd3a2646du, 0x58b47f4du, 0xe9846af9u, 0x6c8e9cf5u};
+  return lane * odd[i];
+}
+
+// y >= 0, at most 448, as one of the two e4m3 values next to it, such that the square is right in the mean:
+// the one that is nearest, q, or the other, o, with probability (y^2 - q^2) / (o^2 - q^2).
+__device__ __forceinline__ float squareByChance(float y, uint32_t dice) {
+  uint32_t e = __builtin_bit_cast(uint32_t, y) & 0x7f800000u;
+  e = e > 0x3c800000u ? e : 0x3c800000u;   // under 2^-6 the codes are as far apart as above
+  const float m = __builtin_bit_cast(float, e + (20u << 23));   // its unit is the codes' step
+  const float q = (y + m) - m, d = y - q;
+  const float step = copysignf(__builtin_bit_cast(float, e - (3u << 23)), d), o = q + step;
+  return (float)dice * fabsf(step * (o + q)) < fabsf(d * (y + q)) * 0x1p32f ? o : q;
+}
+
+// Codes and scale of a run (256 / N lanes, N values each).  SQUARE: the roots of second moments, none above
+// zero with code zero.  Without DICE a rounding to 3 fraction bits is off by at most 2^-4 of the value, and
+// values under 2^-10 of the unit (scale) become zero; with it, by at most twice that, and in the mean by
+// nothing.  Where a value is not finite the scale is NaN, and the codes say nothing.
+template <int N, bool SQUARE, bool DICE>
+__device__ __forceinline__ typename BytesOf<N>::V encode(const typename VecOf<float, N>::F& x, float& scale, uint32_t dice) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < N; i++) {
@@ -136,13 +180,26 @@ __device__ __forceinline__ typename BytesOf<N>::V encode(const typename VecOf<fl
 #pragma unroll
   for (int i = 0; i < N; i++) {
     y[i] = x[i] * inv;
-    if (FLOOR) y[i] = fmaxf(y[i], x[i] > 0.f ? kFp8Min : 0.f);
+    if (SQUARE) y[i] = fmaxf(y[i], x[i] > 0.f ? kFp8Min : 0.f);
+    // (the two roundings of inv may leave the largest a unit above 448; nearest takes that back)
+    if (DICE) y[i] = __builtin_amdgcn_fmed3f(y[i], -kFp8Max, kFp8Max);
+    if (DICE && SQUARE) y[i] = squareByChance(y[i], throwOf(dice, i));
   }
   typename BytesOf<N>::V w;
 #pragma unroll
   for (int h = 0; h < N / 4; h++) {
-    const int c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
-    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], c, true);
+    int c = 0;
+    if constexpr (DICE && !SQUARE) {
+      // the hardware's: it adds the number's upper 20 bits below the last fraction bit and cuts off
+      c = __builtin_amdgcn_cvt_sr_fp8_f32(y[4 * h], throwOf(dice, 4 * h) << 13, c, 0);
+      c = __builtin_amdgcn_cvt_sr_fp8_f32(y[4 * h + 1], throwOf(dice, 4 * h + 1) << 13, c, 1);
+      c = __builtin_amdgcn_cvt_sr_fp8_f32(y[4 * h + 2], throwOf(dice, 4 * h + 2) << 13, c, 2);
+      c = __builtin_amdgcn_cvt_sr_fp8_f32(y[4 * h + 3], throwOf(dice, 4 * h + 3) << 13, c, 3);
+    } else {
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], c, false);
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], c, true);
+    }
+    w[h] = (uint32_t)c;
   }
   return w;
 }
@@ -184,11 +241,12 @@ struct AdamChunk {
   float* mScale;
   float* vScale;
   float coef, invRoot, keep, rate;
+  uint64_t dice;
 };
 
 // A lane's elements of a chunk that begins at `from`.  FULL: the whole chunk is there (so that the loads
 // stand together without branches); else `left` elements are.
-template <class P, class G, bool MASTER, int BITS, bool FULL>
+template <class P, class G, bool MASTER, int BITS, bool DICE, bool FULL>
 __device__ __forceinline__ void adamwChunk(const AdamStepArgs& a, const AdamChunk& t, uint64_t from, int left) {
   constexpr bool wide = MASTER || sizeof(P) == 4 || sizeof(G) == 4;
   constexpr int N = BITS == 8 && !wide ? 8 : 4;
@@ -250,8 +308,9 @@ __device__ __forceinline__ void adamwChunk(const AdamStepArgs& a, const AdamChun
         for (int i = 0; i < N; i++)
           if (i >= n) m[j][i] = r[i] = 0.f;   // behind the tensor's end: no part of the run's scale
       }
-      const auto mw = encode<N, false>(m[j], ms[j]);
-      const auto vw = encode<N, true>(r, vs[j]);
+      const uint32_t dice = DICE ? diceAt(t.dice, mine) : 0;
+      const auto mw = encode<N, false, DICE>(m[j], ms[j], dice);
+      const auto vw = encode<N, true, DICE>(r, vs[j], dice);
       storeBytes<N>((uint8_t*)t.m + at, mw, n);
       storeBytes<N>((uint8_t*)t.v + at, vw, n);
       if ((FULL || n > 0) && threadIdx.x % runLanes == 0) {
@@ -264,7 +323,7 @@ __device__ __forceinline__ void adamwChunk(const AdamStepArgs& a, const AdamChun
 
 // ONE: the step in one launch, every workgroup making what all share by itself.  The last of them to
 // have read the step count advances it.
-template <class P, class G, bool MASTER, int BITS, bool ONE>
+template <class P, class G, bool MASTER, int BITS, bool DICE, bool ONE>
 __global__ void __launch_bounds__(kOpsThreads) adamwKernel(AdamStepArgs a) {
   AdamControl ctl;
   if constexpr (ONE) {
@@ -284,6 +343,7 @@ __global__ void __launch_bounds__(kOpsThreads) adamwKernel(AdamStepArgs a) {
     ctl.invRoot = scalarLoad(&a.ctl->invRoot);
     ctl.lr = scalarLoad(&a.ctl->lr);
     ctl.rate = scalarLoad(&a.ctl->rate);
+    if constexpr (DICE) ctl.t = scalarLoad(&a.ctl->t);
   }
   if (ctl.skip) return;
   constexpr uint32_t chunk = adamChunk(BITS, MASTER || sizeof(P) == 4 || sizeof(G) == 4);
@@ -296,9 +356,10 @@ __global__ void __launch_bounds__(kOpsThreads) adamwKernel(AdamStepArgs a) {
     const double lrScale = scalarLoad(&t->lrScale);
     const AdamChunk k = {scalarLoad(&t->param), scalarLoad(&t->grad), scalarLoad(&t->master), (char*)scalarLoad(&t->m),
                          (char*)scalarLoad(&t->v), scalarLoad(&t->mScale), scalarLoad(&t->vScale), ctl.coef, ctl.invRoot,
-                         (float)(1.0 - ctl.lr * lrScale * scalarLoad(&t->decay)), (float)(ctl.rate * lrScale)};
-    if (left >= chunk) adamwChunk<P, G, MASTER, BITS, true>(a, k, from, 0);
-    else adamwChunk<P, G, MASTER, BITS, false>(a, k, from, (int)left);
+                         (float)(1.0 - ctl.lr * lrScale * scalarLoad(&t->decay)), (float)(ctl.rate * lrScale),
+                         DICE ? diceOf(a.seed, (uint64_t)ctl.t, c) : 0};
+    if (left >= chunk) adamwChunk<P, G, MASTER, BITS, DICE, true>(a, k, from, 0);
+    else adamwChunk<P, G, MASTER, BITS, DICE, false>(a, k, from, (int)left);
   }
 }
 
@@ -308,46 +369,52 @@ __global__ void __launch_bounds__(kOpsThreads) adamwKernel(AdamStepArgs a) {
 // 6.3 against 7.6 and 6.5 against 4.8, 512 29 against 7.
 constexpr uint32_t kOneLaunch = 32;
 
-template <class P, class G, bool MASTER, int BITS>
+template <class P, class G, bool MASTER, int BITS, bool DICE>
 static int launchStep(const AdamStepArgs& a, void* stream) {
   constexpr uint32_t most = 1u << 20;   // a launch's threads are counted in 32 bits
   const uint32_t grid = a.tab.chunks < most ? a.tab.chunks : most;
   if (grid && grid <= kOneLaunch) {
-    hipLaunchKernelGGL((adamwKernel<P, G, MASTER, BITS, true>), dim3(grid), dim3(kOpsThreads), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((adamwKernel<P, G, MASTER, BITS, DICE, true>), dim3(grid), dim3(kOpsThreads), 0, (hipStream_t)stream, a);
     return hipGetLastError() == hipSuccess ? 0 : 1;
   }
   hipLaunchKernelGGL(adamwBeginKernel, dim3(1), dim3(1), 0, (hipStream_t)stream, a);
   if (hipGetLastError() != hipSuccess) return 1;
   if (grid == 0) return 0;
-  hipLaunchKernelGGL((adamwKernel<P, G, MASTER, BITS, false>), dim3(grid), dim3(kOpsThreads), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL((adamwKernel<P, G, MASTER, BITS, DICE, false>), dim3(grid), dim3(kOpsThreads), 0, (hipStream_t)stream, a);
   return hipGetLastError() == hipSuccess ? 0 : 1;
 }
 
+template <class P, class G, bool MASTER>
+static int launchBits(const AdamStepArgs& a, int bits, bool dice, void* stream) {
+  if (bits == 32) return launchStep<P, G, MASTER, 32, false>(a, stream);
+  return dice ? launchStep<P, G, MASTER, 8, true>(a, stream) : launchStep<P, G, MASTER, 8, false>(a, stream);
+}
+
 template <class P, class G>
-static int launchState(const AdamStepArgs& a, bool master, int bits, void* stream) {
+static int launchState(const AdamStepArgs& a, bool master, int bits, bool dice, void* stream) {
   if constexpr (__is_same(P, float)) {
     if (master) return 1;
   } else {
-    if (master) return bits == 32 ? launchStep<P, G, true, 32>(a, stream) : launchStep<P, G, true, 8>(a, stream);
+    if (master) return launchBits<P, G, true>(a, bits, dice, stream);
   }
-  return bits == 32 ? launchStep<P, G, false, 32>(a, stream) : launchStep<P, G, false, 8>(a, stream);
+  return launchBits<P, G, false>(a, bits, dice, stream);
 }
 
 template <class P>
-static int launchGrad(const AdamStepArgs& a, int gradType, bool master, int bits, void* stream) {
+static int launchGrad(const AdamStepArgs& a, int gradType, bool master, int bits, bool dice, void* stream) {
   switch (gradType) {
-    case 6: return launchState<P, _Float16>(a, master, bits, stream);
-    case 7: return launchState<P, float>(a, master, bits, stream);
-    case 9: return launchState<P, __bf16>(a, master, bits, stream);
+    case 6: return launchState<P, _Float16>(a, master, bits, dice, stream);
+    case 7: return launchState<P, float>(a, master, bits, dice, stream);
+    case 9: return launchState<P, __bf16>(a, master, bits, dice, stream);
   }
   return 1;
 }
 
-int launchAdamW(const AdamStepArgs& a, int paramType, int gradType, bool master, int bits, void* stream) {
+int launchAdamW(const AdamStepArgs& a, int paramType, int gradType, bool master, int bits, bool dice, void* stream) {
   switch (paramType) {
-    case 6: return launchGrad<_Float16>(a, gradType, master, bits, stream);
-    case 7: return launchGrad<float>(a, gradType, master, bits, stream);
-    case 9: return launchGrad<__bf16>(a, gradType, master, bits, stream);
+    case 6: return launchGrad<_Float16>(a, gradType, master, bits, dice, stream);
+    case 7: return launchGrad<float>(a, gradType, master, bits, dice, stream);
+    case 9: return launchGrad<__bf16>(a, gradType, master, bits, dice, stream);
   }
   return 1;
 }

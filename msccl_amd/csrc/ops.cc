@@ -95,6 +95,8 @@ struct mscclAmdAdamWPlan {
   TensorTable<AdamTensor> tab;
   std::vector<size_t> counts;
   std::vector<Range> written;   // sorted
+  bool dice = false;            // states of 8 bits rounded by chance
+  uint64_t seed = 0;
 };
 
 extern "C" {
@@ -249,6 +251,16 @@ ncclResult_t mscclAmdAdamWCreate(mscclAmdAdamW_t* plan, const mscclAmdAdamWTenso
   return ncclSuccess;
 }
 
+ncclResult_t mscclAmdAdamWSetRounding(mscclAmdAdamW_t plan, mscclAmdRounding_t rounding, uint64_t seed) {
+  const char* name = "mscclAmdAdamWSetRounding";
+  if (!plan || plan->magic != kAdamMagic) REFUSE("%s : invalid plan", name);
+  if (rounding != mscclAmdNearest && rounding != mscclAmdStochastic) REFUSE("%s : invalid rounding %d", name, (int)rounding);
+  if (rounding == mscclAmdStochastic && plan->bits != 8) REFUSE("%s : states of %d bits are rounded to nearest", name, plan->bits);
+  plan->dice = rounding == mscclAmdStochastic;
+  plan->seed = seed;
+  return ncclSuccess;
+}
+
 ncclResult_t mscclAmdAdamWSetGrads(mscclAmdAdamW_t plan, const void* const* grads, size_t n, hipStream_t stream) {
   const char* name = "mscclAmdAdamWSetGrads";
   if (!plan || plan->magic != kAdamMagic) REFUSE("%s : invalid plan", name);
@@ -296,7 +308,8 @@ ncclResult_t mscclAmdAdamWStep(mscclAmdAdamW_t plan, double lr, const float* lrD
   a.b2 = (float)beta2;
   a.c2 = (float)(1.0 - beta2);
   a.eps = (float)eps;
-  if (launchAdamW(a, plan->paramType, plan->gradType, plan->master, plan->bits, stream)) {
+  a.seed = plan->seed;
+  if (launchAdamW(a, plan->paramType, plan->gradType, plan->master, plan->bits, plan->dice, stream)) {
     WARN("%s : launch failed", name);
     return ncclUnhandledCudaError;
   }

@@ -13,6 +13,7 @@ TypeError here, or NcclError from the library.
 """
 import ctypes
 import struct
+import warnings
 from typing import Optional, Sequence, Union
 
 import torch
@@ -22,6 +23,7 @@ from . import BFLOAT16, FLOAT16, FLOAT32, FLOAT64, INT32, INT64, Comm, NcclError
 _TYPES = {torch.float32: FLOAT32, torch.float16: FLOAT16, torch.bfloat16: BFLOAT16}
 _INDEX = {torch.int32: INT32, torch.int64: INT64}
 _SCORES = {"softmax": 0, "sigmoid": 1}
+_ROUNDINGS = {"nearest": 0, "stochastic": 1}
 STATE_BLOCK = 256  # elements that share a scale in 8-bit states
 
 
@@ -49,6 +51,7 @@ def _lib():
         L.mscclAmdAdamWBytes.argtypes = [sz]
         L.mscclAmdAdamWBytes.restype = sz
         L.mscclAmdAdamWCreate.argtypes = [ctypes.POINTER(vp), ctypes.c_char_p, sz, i, i, i, vp, vp, sz, vp]
+        L.mscclAmdAdamWSetRounding.argtypes = [vp, i, ctypes.c_uint64]
         L.mscclAmdAdamWSetGrads.argtypes = [vp, vp, sz, vp]
         L.mscclAmdAdamWStep.argtypes = [vp, d, vp, d, d, d, d, vp, d, vp]
         L.mscclAmdAdamWDestroy.argtypes = [vp]
@@ -218,14 +221,22 @@ class AdamW(_Plan):
     a tensor (the last may be shorter); adamw_state makes them.  step: one int64, the steps taken so far,
     this plan's own.  weight_decay, lr_scale: a number, or one for each tensor.  Tensors may have any size
     and start anywhere; they must not overlap (a weight that layers share is listed once).  Steps of one
-    plan must be ordered after each other."""
+    plan must be ordered after each other.
+
+    rounding, seed: how 8-bit states are rounded.  "stochastic" is right in the mean over any number of
+    steps; one element's sqrt(exp_avg_sq) is then within about a sixth of the 32-bit state's.  "nearest" is
+    closer within a step but never follows what changes by less than half a code's step (3.1 to 6.3 %) in
+    each: second moments neither decay by themselves nor stay when a neighbour's growth raises their scale,
+    and drift to many times their value over thousands of steps at beta2 of 0.94 and more (mscclAmdAdamWSetRounding).
+    None is nearest, with a warning at the first such step."""
     _destroy = "mscclAmdAdamWDestroy"
 
     def __init__(self, params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
                  exp_avg_sqs: Sequence[torch.Tensor], step: torch.Tensor, masters: Optional[Sequence[torch.Tensor]] = None,
                  exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
                  exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None,
-                 weight_decay: Union[float, Sequence[float]] = 0.0, lr_scale: Union[float, Sequence[float]] = 1.0):
+                 weight_decay: Union[float, Sequence[float]] = 0.0, lr_scale: Union[float, Sequence[float]] = 1.0,
+                 rounding: Optional[str] = None, seed: int = 0):
         super().__init__()
         n = len(params)
         if not n:
@@ -236,6 +247,12 @@ class AdamW(_Plan):
             raise ValueError("8-bit states need their scales")
         if bits == 32 and (exp_avg_scales is not None or exp_avg_sq_scales is not None):
             raise ValueError("32-bit states have no scales")
+        if rounding is not None and rounding not in _ROUNDINGS:
+            raise ValueError("rounding %r is not one of %s" % (rounding, ", ".join(_ROUNDINGS)))
+        if rounding == "stochastic" and bits != 8:
+            raise ValueError("32-bit states are rounded to nearest")
+        if not 0 <= seed < 1 << 64:
+            raise ValueError("seed %r is not a 64-bit number" % (seed,))
         decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * n
         rates = list(lr_scale) if isinstance(lr_scale, (list, tuple)) else [lr_scale] * n
         state = (torch.float8_e4m3fn,) if bits == 8 else (torch.float32,)
@@ -268,7 +285,10 @@ class AdamW(_Plan):
             _check(L.mscclAmdAdamWCreate(ctypes.byref(self.handle), rows, n, _TYPES[params[0].dtype],
                                          _TYPES[grads[0].dtype], bits, step.data_ptr(), self.table.data_ptr(),
                                          self.table.numel(), _stream(dev)), "mscclAmdAdamWCreate")
+            if rounding == "stochastic":
+                _check(L.mscclAmdAdamWSetRounding(self.handle, _ROUNDINGS[rounding], seed), "mscclAmdAdamWSetRounding")
             self._ready()
+        self._unsaid = bits == 8 and rounding is None
 
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
         """Other gradient tensors (same sizes and type) for the steps enqueued from now on; the earlier
@@ -302,6 +322,11 @@ class AdamW(_Plan):
             total = grad_square_sum.data_ptr()
         if max_norm is not None and not max_norm > 0:
             raise ValueError("max_norm must be above zero")
+        if self._unsaid and betas[1] > 0.9375:   # a root of v decays by 1 - sqrt(beta2), half a code's step is 2^-5 or more
+            self._unsaid = False
+            warnings.warn("AdamW: second moments of 8 bits that are rounded to nearest drift over many steps with beta2 %g; "
+                          "rounding=\"stochastic\" follows them (rounding=\"nearest\" says that this is meant)" % betas[1],
+                          stacklevel=2)
         launch, args = _lib().mscclAmdAdamWStep, (self.handle, lr, at, betas[0], betas[1], eps, grad_scale, total,
                                                   max_norm or 0.0, stream)
         if _elsewhere(self.device):

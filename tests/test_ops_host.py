@@ -214,3 +214,10 @@ int main(void) {
                     "-D__HIP_PLATFORM_AMD__", str(src), "-o", exe], check=True, capture_output=True, text=True)
     got = [int(x) for x in subprocess.run([exe], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [ops._TENSOR.size, ops._TENSOR.size - 8, ops._ROUTER.size - 4, 56, 56]
+
+
+def test_adamw_set_rounding_refuses_bad_plan():
+    L = ops._lib()
+    junk = ctypes.create_string_buffer(256)
+    for h in (None, ctypes.addressof(junk)):
+        assert L.mscclAmdAdamWSetRounding(h, 1, 0) == BAD
