@@ -389,6 +389,29 @@ def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: S
 
 # ---- balance loss of a router's experts ----------------------------------------------------------
 
+class _Stats(torch.autograd.Function):
+    """balance_stats of logits that need a gradient: their sums are tied to them, and backward says what is missing."""
+
+    @staticmethod
+    def forward(ctx, logits, index, valid, score):
+        counts, probs = balance_stats(logits, index, valid, score)
+        ctx.mark_non_differentiable(counts)
+        return counts, probs
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("the balance loss's gradient is balance_backward's: add that to the logits' gradient, and leave "
+                           "the loss out of backward (detach it)")
+
+
+class _Loss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, counts, probs, top_k, coef):
+        return balance_loss(counts, probs, top_k, coef)
+
+    backward = _Stats.backward
+
+
 def _rows(t: torch.Tensor, what: str, rows: int, cols: int) -> int:
     """The stride from row to row of a matrix whose rows are whole and apart."""
     down, along = t.stride()
@@ -430,9 +453,12 @@ def balance_stats(logits: torch.Tensor, index: torch.Tensor, valid: Optional[tor
     """(counts, probs) of a router's choice: counts int64 [experts + 1], the slots of valid tokens that chose
     each expert and then the number of valid tokens; probs float32 [experts], the sums over valid tokens of
     softmax(logits), or with score="sigmoid" of sigmoid(logits) over its row's sum.  index [tokens, k]: the
-    chosen experts (one outside [0, experts) is a dropped slot); valid [tokens]: None, or false for padding."""
+    chosen experts (one outside [0, experts) is a dropped slot); valid [tokens]: None, or false for padding.
+    The gradient is balance_backward's, not autograd's: backward through probs of logits that need one raises."""
     if index is None:
         raise TypeError("index must be [tokens, k] of int32 or int64")
+    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
+        return _Stats.apply(logits, index, valid, score)
     r = _router(logits, index, 0, valid, score)
     dev = logits.device
     if _elsewhere(dev):
@@ -467,8 +493,11 @@ def balance_all_reduce(comms: Sequence[Comm], counts: Sequence[torch.Tensor], pr
 
 
 def balance_loss(counts: torch.Tensor, probs: torch.Tensor, top_k: int, coef: float = 1.0) -> torch.Tensor:
-    """coef * experts / (k N^2) * sum of counts[e] * probs[e] (N valid tokens; 0 for none), float32 of one element."""
+    """coef * experts / (k N^2) * sum of counts[e] * probs[e] (N valid tokens; 0 for none), float32 of one element.
+    Its gradient at the logits is balance_backward's, not autograd's (see balance_stats)."""
     _flat(probs, "probs", (torch.float32,))
+    if probs.requires_grad and torch.is_grad_enabled():
+        return _Loss.apply(counts, probs, top_k, coef)
     dev, e = probs.device, probs.numel()
     _flat(counts, "counts", (torch.int64,), dev, e + 1)
     if not 0 < top_k <= e:
