@@ -104,12 +104,23 @@ def _inside(span, at: int, nbytes: int) -> bool:
     return span is None or (at <= span[0] and span[1] <= at + nbytes)
 
 
+def _changed(tensors) -> None:
+    """Tells autograd that a kernel wrote these: a graph that holds their old values refuses to use the new ones."""
+    torch._C._increment_version(tensors)
+
+
+def _versions(tensors):
+    """One of these for each version counter (views share their base's)."""
+    return list({id(t if t._base is None else t._base): t for t in tensors}.values())
+
+
 class _Plan:
     """A plan's handle, its device memory and the tensors whose addresses it holds."""
     _destroy = ""
 
     def __init__(self):
         self.handle = ctypes.c_void_p()
+        self._weights = None
 
     def _memory(self, device, nbytes: int):
         if torch.cuda.is_current_stream_capturing():
@@ -137,7 +148,7 @@ class _Plan:
             h, self.handle = self.handle, ctypes.c_void_p()
             _check(getattr(_lib(), self._destroy)(h), self._destroy)
         self.table = None
-        self.tensors = None
+        self.tensors = self._weights = None
 
     def __del__(self):
         try:
@@ -185,12 +196,15 @@ class SquareSum(_Plan):
                 return self(out)
         # scratch of this call's own: calls on several streams, or in several graphs, do not meet in it
         scratch = torch.empty(self._scratch, dtype=torch.uint8, device=dev) if self._scratch else None
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty(1, dtype=torch.float64, device=dev)
         rc = _lib().mscclAmdSquareSum(self.handle, out.data_ptr(), scratch.data_ptr() if self._scratch else None,
                                       self._scratch, stream)
         if rc:
             raise NcclError(rc, "mscclAmdSquareSum")
+        if given:
+            _changed((out,))
         return out
 
 
@@ -289,6 +303,7 @@ class AdamW(_Plan):
                 _check(L.mscclAmdAdamWSetRounding(self.handle, _ROUNDINGS[rounding], seed), "mscclAmdAdamWSetRounding")
             self._ready()
         self._unsaid = bits == 8 and rounding is None
+        self._weights = _versions(list(params) + list(masters or ()))
 
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
         """Other gradient tensors (same sizes and type) for the steps enqueued from now on; the earlier
@@ -336,6 +351,7 @@ class AdamW(_Plan):
             rc = launch(*args)
         if rc:
             raise NcclError(rc, "mscclAmdAdamWStep")
+        _changed(self._weights)
 
 
 def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: Sequence[torch.Tensor],
@@ -384,6 +400,7 @@ def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: S
         for r, c in enumerate(comms):
             base = params[r].data_ptr()
             c.all_gather(base + c.rank * block * es, base, block, pt, stream=_stream(params[r].device))
+    _changed(list(shards) + list(params))
     return totals
 
 
@@ -490,6 +507,7 @@ def balance_all_reduce(comms: Sequence[Comm], counts: Sequence[torch.Tensor], pr
         with group():
             for r, c in enumerate(comms):
                 c.all_reduce(ts[r].data_ptr(), ts[r].data_ptr(), ts[r].numel(), code, stream=_stream(ts[r].device))
+        _changed(list(ts))
 
 
 def balance_loss(counts: torch.Tensor, probs: torch.Tensor, top_k: int, coef: float = 1.0) -> torch.Tensor:
@@ -522,7 +540,7 @@ def balance_backward(logits: torch.Tensor, counts: torch.Tensor, top_k: int, coe
     dev = logits.device
     t, e = logits.shape
     _flat(counts, "counts", (torch.int64,), dev, e + 1)
-    up = None
+    up, given = None, out is not None
     if grad_output is not None:
         _flat(grad_output, "grad_output", (torch.float32,), dev, 1)
         up = grad_output.data_ptr()
@@ -543,6 +561,8 @@ def balance_backward(logits: torch.Tensor, counts: torch.Tensor, top_k: int, coe
         rc = launch(*args)
     if rc:
         raise NcclError(rc, "mscclAmdBalanceBackward")
+    if given:
+        _changed((out,))
     return out
 
 
