@@ -127,19 +127,26 @@ class _Plan:
             raise RuntimeError("make the plan before the capture")
         self.device = device
         self.table = torch.empty(max(8, nbytes), dtype=torch.uint8, device=device)
-        self._home = _stream(device)
+        self._streams = {}   # those that had a call
 
     def _ready(self):
         # the table was written on this stream; the plan may be used on any
+        self._live()
         torch.cuda.current_stream(self.device).synchronize()
+
+    def _held(self):
+        return [self.table] + self.tensors
 
     def _live(self) -> int:
         """The stream of a call on the plan."""
         if not self.handle:
             raise ValueError("the plan is closed")
         s = _stream(self.device)
-        if s != self._home:  # the table's memory is not to be used again before this stream is done with it
-            self.table.record_stream(torch.cuda.current_stream(self.device))
+        if s not in self._streams:
+            # whoever drops the plan or its tensors: their memory is not used again before this stream is done
+            self._streams[s] = stream = torch.cuda.current_stream(self.device)
+            for t in _versions(self._held()):
+                t.record_stream(stream)
         return s
 
     def close(self) -> None:
@@ -305,6 +312,9 @@ class AdamW(_Plan):
         self._unsaid = bits == 8 and rounding is None
         self._weights = _versions(list(params) + list(masters or ()))
 
+    def _held(self):
+        return [self.table] + [t for ts in self.tensors[:-1] if ts for t in ts] + self.tensors[-1:]
+
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
         """Other gradient tensors (same sizes and type) for the steps enqueued from now on; the earlier
         steps must be on the current stream or ordered before it."""
@@ -317,6 +327,9 @@ class AdamW(_Plan):
         ptrs = (ctypes.c_void_p * len(grads))(*[g.data_ptr() for g in grads])
         with torch.cuda.device(self.device):
             _check(_lib().mscclAmdAdamWSetGrads(self.handle, ptrs, len(grads), stream), "mscclAmdAdamWSetGrads")
+        for s in self._streams.values():
+            for g in grads:
+                g.record_stream(s)
         self.tensors[1] = list(grads)
         self.grad_span = _span(grads)
 
