@@ -102,7 +102,8 @@ typedef enum { mscclAmdNearest = 0, mscclAmdStochastic = 1 } mscclAmdRounding_t;
 ncclResult_t mscclAmdAdamWSetRounding(mscclAmdAdamW_t plan, mscclAmdRounding_t rounding, uint64_t seed);
 
 /* Other gradient buffers for all n tensors (host array of device addresses, read now), from `stream`'s
- * next step on. */
+ * next step on.  Captured into a graph it changes them when the graph runs: until then steps read the
+ * buffers from before, and every replay sets these again, so both have to live as long. */
 ncclResult_t mscclAmdAdamWSetGrads(mscclAmdAdamW_t plan, const void* const* grads, size_t n, hipStream_t stream);
 
 /* One step, with t the advanced step count and g = c * grad:

@@ -155,7 +155,7 @@ class _Plan:
             h, self.handle = self.handle, ctypes.c_void_p()
             _check(getattr(_lib(), self._destroy)(h), self._destroy)
         self.table = None
-        self.tensors = self._weights = None
+        self.tensors = self._weights = self._captured = None
 
     def __del__(self):
         try:
@@ -311,13 +311,15 @@ class AdamW(_Plan):
             self._ready()
         self._unsaid = bits == 8 and rounding is None
         self._weights = _versions(list(params) + list(masters or ()))
+        self._captured = []
 
     def _held(self):
         return [self.table] + [t for ts in self.tensors[:-1] if ts for t in ts] + self.tensors[-1:]
 
     def set_grads(self, grads: Sequence[torch.Tensor]) -> None:
         """Other gradient tensors (same sizes and type) for the steps enqueued from now on; the earlier
-        steps must be on the current stream or ordered before it."""
+        steps must be on the current stream or ordered before it.  Captured, it changes them at each replay
+        and not before: the plan then keeps the earlier ones too."""
         stream = self._live()
         params = self.tensors[0]
         if len(grads) != len(params):
@@ -330,6 +332,10 @@ class AdamW(_Plan):
         for s in self._streams.values():
             for g in grads:
                 g.record_stream(s)
+        with torch.cuda.device(self.device):
+            captured = torch.cuda.is_current_stream_capturing()
+        if captured:   # until a replay the table holds the earlier ones, and a later call does not end the replays
+            self._captured.append((self.tensors[1], list(grads)))
         self.tensors[1] = list(grads)
         self.grad_span = _span(grads)
 

@@ -68,3 +68,49 @@ def test_steps_outlive_their_dropped_gradients():
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(p, want))
     del junk
+
+
+def test_captured_gradients_live_as_long_as_the_plan():
+    """Until the graph runs the table holds the gradients from before, and each replay sets the captured ones."""
+    import gc
+    import weakref
+    n = 3000
+    first, second, third = ([torch.randn(n, generator=gen(k), device="cuda")] for k in (1, 2, 3))
+    values = [x[0].clone() for x in (first, second, third)]
+    a, b = torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    plans, grad = [], torch.zeros(n, device="cuda")
+    for p, g in ((a, first), (b, [grad])):
+        m, v = ops.adamw_state(p)
+        plans.append(ops.AdamW([p], g, [m], [v], torch.zeros(1, dtype=torch.int64, device="cuda")))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        plans[0].set_grads(second)
+        plans[0].step(1e-2)
+    alive = [weakref.ref(x[0]) for x in (first, second)]
+    del first, second
+    gc.collect()
+    assert all(r() is not None for r in alive)
+
+    def same(k):
+        grad.copy_(values[k])
+        plans[1].step(1e-2)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+    plans[0].step(1e-2)      # not replayed yet: the first
+    same(0)
+    graph.replay()           # the second
+    same(1)
+    plans[0].set_grads(third)
+    gc.collect()
+    plans[0].step(1e-2)
+    same(2)
+    graph.replay()           # the second again, and from there on
+    same(1)
+    plans[0].step(1e-2)
+    same(1)
+    assert all(r() is not None for r in alive)
+    torch.cuda.synchronize()
+    plans[0].close()
+    gc.collect()
+    assert all(r() is None for r in alive)
