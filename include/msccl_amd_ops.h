@@ -121,6 +121,10 @@ ncclResult_t mscclAmdAdamWStep(mscclAmdAdamW_t plan, double lr, const float* lrD
                                double eps, double gradScale, const double* gradSquareSum, double maxNorm,
                                hipStream_t stream);
 
+/* What mscclAmdAdamWStep says to these numbers, without a step: for callers that have to know before they
+ * join a collective. */
+ncclResult_t mscclAmdAdamWCheck(double lr, double beta1, double beta2, double eps, double gradScale, double maxNorm);
+
 ncclResult_t mscclAmdAdamWDestroy(mscclAmdAdamW_t plan);
 
 /* ---- balance loss of a router's experts ----------------------------------------------------- */

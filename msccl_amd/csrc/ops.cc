@@ -280,16 +280,25 @@ ncclResult_t mscclAmdAdamWSetGrads(mscclAmdAdamW_t plan, const void* const* grad
   return ncclSuccess;
 }
 
-ncclResult_t mscclAmdAdamWStep(mscclAmdAdamW_t plan, double lr, const float* lrDevice, double beta1, double beta2,
-                               double eps, double gradScale, const double* gradSquareSum, double maxNorm,
-                               hipStream_t stream) {
-  const char* name = "mscclAmdAdamWStep";
-  if (!plan || plan->magic != kAdamMagic) REFUSE("%s : invalid plan", name);
+static ncclResult_t checkNumbers(const char* name, double lr, double beta1, double beta2, double eps, double gradScale, double maxNorm) {
   if (!std::isfinite(lr)) REFUSE("%s : lr is not finite", name);
   if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1)) REFUSE("%s : betas (%g, %g) outside [0, 1)", name, beta1, beta2);
   if (!(eps == 0 || (eps >= FLT_MIN && eps <= FLT_MAX))) REFUSE("%s : eps %g (0, or a normal 32-bit value)", name, eps);
   if (!(gradScale >= FLT_MIN && gradScale <= FLT_MAX)) REFUSE("%s : gradScale %g (a normal 32-bit value above zero)", name, gradScale);
   if (!(maxNorm >= 0)) REFUSE("%s : maxNorm %g", name, maxNorm);
+  return ncclSuccess;
+}
+
+ncclResult_t mscclAmdAdamWCheck(double lr, double beta1, double beta2, double eps, double gradScale, double maxNorm) {
+  return checkNumbers("mscclAmdAdamWCheck", lr, beta1, beta2, eps, gradScale, maxNorm);
+}
+
+ncclResult_t mscclAmdAdamWStep(mscclAmdAdamW_t plan, double lr, const float* lrDevice, double beta1, double beta2,
+                               double eps, double gradScale, const double* gradSquareSum, double maxNorm,
+                               hipStream_t stream) {
+  const char* name = "mscclAmdAdamWStep";
+  if (!plan || plan->magic != kAdamMagic) REFUSE("%s : invalid plan", name);
+  NCCLCHECK(checkNumbers(name, lr, beta1, beta2, eps, gradScale, maxNorm));
   if (maxNorm > 0 && !gradSquareSum) REFUSE("%s : maxNorm without a square sum", name);
   if (!aligned(gradSquareSum, 8) || !aligned(lrDevice, 4)) REFUSE("%s : gradSquareSum or lrDevice is not aligned", name);
   AdamStepArgs a;

@@ -54,6 +54,7 @@ def _lib():
         L.mscclAmdAdamWSetRounding.argtypes = [vp, i, ctypes.c_uint64]
         L.mscclAmdAdamWSetGrads.argtypes = [vp, vp, sz, vp]
         L.mscclAmdAdamWStep.argtypes = [vp, d, vp, d, d, d, d, vp, d, vp]
+        L.mscclAmdAdamWCheck.argtypes = [d, d, d, d, d, d]
         L.mscclAmdAdamWDestroy.argtypes = [vp]
         L.mscclAmdBalanceWorkspace.argtypes = [sz, sz]
         L.mscclAmdBalanceWorkspace.restype = sz
@@ -339,6 +340,17 @@ class AdamW(_Plan):
         self.tensors[1] = list(grads)
         self.grad_span = _span(grads)
 
+    def _check_step(self, lr, betas, eps, grad_scale, max_norm) -> None:
+        """What step and the library refuse, without a step."""
+        if not self.handle:
+            raise ValueError("the plan is closed")
+        if isinstance(lr, torch.Tensor):
+            _flat(lr, "lr", (torch.float32,), self.device, 1)
+            lr = 0.0
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError("max_norm must be above zero")
+        _check(_lib().mscclAmdAdamWCheck(lr, betas[0], betas[1], eps, grad_scale, max_norm or 0.0), "mscclAmdAdamWCheck")
+
     def step(self, lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8, grad_scale: float = 1.0,
              grad_square_sum: Optional[torch.Tensor] = None, max_norm: Optional[float] = None) -> None:
         """One step (the formulas: mscclAmdAdamWStep).  lr: a number, or a float32 tensor of one element,
@@ -387,7 +399,14 @@ def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: S
     sqrt(sum) / nranks)."""
     if not len(comms) == len(grads) == len(shards) == len(params) == len(plans) == len(sums) or not comms:
         raise ValueError("one gradient, shard, weight buffer, plan and square sum for each communicator")
+    # all of it before the first collective, for which other ranks would wait: a step that is refused
+    # afterwards would leave them waiting, and some plans a step ahead of others
+    rates = list(lr) if isinstance(lr, (list, tuple)) else [lr] * len(comms)
+    if len(rates) != len(comms):
+        raise ValueError("lr: a number, or one for each communicator")
     n = comms[0].nranks
+    for p, x in zip(plans, rates):
+        p._check_step(x, betas, eps, 1.0 / n, max_norm)
     for r, c in enumerate(comms):
         block = shards[r].numel()
         dev = torch.device("cuda", c.device)
@@ -396,8 +415,14 @@ def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: S
         _flat(params[r], "params[%d]" % r, (params[0].dtype,) if params[0].dtype in _TYPES else tuple(_TYPES), dev, n * block)
         if shards[r].dtype != shards[0].dtype or block != shards[0].numel():
             raise ValueError("the shards must have one size and type")
+        if not sums[r].handle:
+            raise ValueError("sums[%d] is closed" % r)
         if plans[r].device != dev or sums[r].device != dev:
             raise ValueError("plans[%d] or sums[%d] is on another device than its communicator" % (r, r))
+        if plans[r]._grad_type != shards[r].dtype or sums[r].tensors[0].dtype != shards[r].dtype:
+            raise TypeError("plans[%d] or sums[%d] reads gradients of another type than shards[%d]'s" % (r, r, r))
+        if plans[r].tensors[0][0].dtype != params[r].dtype:
+            raise TypeError("plans[%d] writes weights of another type than params[%d]'s" % (r, r))
         size = block * shards[r].element_size()
         if not (_inside(plans[r].grad_span, shards[r].data_ptr(), size) and _inside(sums[r].span, shards[r].data_ptr(), size)):
             raise ValueError("plans[%d] or sums[%d] reads gradients outside shards[%d]" % (r, r, r))
@@ -414,7 +439,7 @@ def sharded_step(comms: Sequence[Comm], grads: Sequence[torch.Tensor], shards: S
         for r, c in enumerate(comms):
             c.all_reduce(totals[r].data_ptr(), totals[r].data_ptr(), 1, FLOAT64, stream=_stream(totals[r].device))
     for r, p in enumerate(plans):
-        p.step(lr[r] if isinstance(lr, (list, tuple)) else lr, betas, eps, 1.0 / n, totals[r], max_norm)
+        p.step(rates[r], betas, eps, 1.0 / n, totals[r], max_norm)
     with group():
         for r, c in enumerate(comms):
             base = params[r].data_ptr()

@@ -1,0 +1,70 @@
+"""A sharded training step refuses what it refuses before its first collective."""
+import pytest
+import torch
+
+import msccl_amd as M
+from msccl_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+class Ranks:
+    def __init__(self, comms, dtype=torch.bfloat16, block=512):
+        n = len(comms)
+        self.comms, self.block = comms, block
+        self.params = [torch.ones(n * block, dtype=dtype, device="cuda") for _ in range(n)]
+        self.grads = [torch.ones(n * block, dtype=dtype, device="cuda") for _ in range(n)]
+        self.shards = [torch.zeros(block, dtype=dtype, device="cuda") for _ in range(n)]
+        self.plans, self.sums, self.state = [], [], []
+        for r in range(n):
+            plan, state = self.plan(r, self.params[r][r * block:(r + 1) * block], self.shards[r])
+            self.plans.append(plan)
+            self.state += state
+            self.sums.append(ops.SquareSum([self.shards[r]]))
+
+    def plan(self, r, p, g):
+        m, v = ops.adamw_state(p)
+        step = torch.zeros(1, dtype=torch.int64, device="cuda")
+        return ops.AdamW([p], [g], [m], [v], step), [m, v, step]
+
+    def go(self, **kw):
+        args = dict(comms=self.comms, grads=self.grads, shards=self.shards, params=self.params, plans=self.plans, sums=self.sums, lr=1e-2)
+        return ops.sharded_step(**(args | kw))
+
+
+def test_nothing_has_run_when_a_step_is_refused(monkeypatch):
+    comms = M.Comm.init_all([0, 0])
+    try:
+        k = Ranks(comms)
+        lr = torch.full((1,), 1e-2, device="cuda")
+        closed, _ = k.plan(1, k.params[1][512:], k.shards[1])
+        closed.close()
+        gone = ops.SquareSum([k.shards[1]])
+        gone.close()
+        half = k.shards[1].view(torch.float16)
+        other_type, keep = k.plan(1, k.params[1][512:], half)
+        other_weights, also = k.plan(1, k.params[1][512:].view(torch.float16), k.shards[1])
+        called = []
+        for name in ("reduce_scatter", "all_reduce", "all_gather"):
+            real = getattr(M.Comm, name)
+            monkeypatch.setattr(M.Comm, name, lambda *a, _r=real, _n=name, **kw: (called.append(_n), _r(*a, **kw))[1])
+        bad = [dict(lr=[1e-2]), dict(lr=[lr] * 3), dict(lr=float("nan")), dict(lr=[1e-2, float("inf")]), dict(lr=lr.double()), dict(lr=[lr, lr.cpu()]),
+               dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(eps=-1.0), dict(max_norm=0.0), dict(max_norm=-1.0),
+               dict(max_norm=float("nan")), dict(plans=[k.plans[0], closed]), dict(sums=[k.sums[0], gone]),
+               dict(plans=[k.plans[0], other_type]), dict(sums=[k.sums[0], ops.SquareSum([half])]),
+               dict(plans=[k.plans[0], other_weights])]
+        old = [t.clone() for t in k.shards + k.params + k.state]
+        for kw in bad:
+            with pytest.raises((ValueError, TypeError, ops.NcclError)):
+                k.go(**kw)
+            torch.cuda.synchronize()
+            assert called == [] and all(torch.equal(a, b) for a, b in zip(old, k.shards + k.params + k.state)), kw
+        for kw in (dict(), dict(lr=[1e-2, 2e-2]), dict(lr=lr), dict(lr=(lr, lr), max_norm=1.0)):
+            k.go(**kw)
+        torch.cuda.synchronize()
+        assert called == ["reduce_scatter", "reduce_scatter", "all_reduce", "all_reduce", "all_gather", "all_gather"] * 4
+        assert [int(k.state[i]) for i in (2, 5)] == [4, 4] and torch.equal(k.params[0], k.params[1])
+    finally:
+        torch.cuda.synchronize()
+        for c in comms:
+            c.destroy()

@@ -221,3 +221,17 @@ def test_adamw_set_rounding_refuses_bad_plan():
     junk = ctypes.create_string_buffer(256)
     for h in (None, ctypes.addressof(junk)):
         assert L.mscclAmdAdamWSetRounding(h, 1, 0) == BAD
+
+
+def test_adamw_check_is_the_steps():
+    """The numbers that a step refuses, without a plan; a chain of collectives asks before its first."""
+    L = ops._lib()
+    good = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, scale=0.5, norm=0.0)
+    check = lambda **kw: L.mscclAmdAdamWCheck(*(good | kw).values())  # noqa: E731
+    for kw in (dict(), dict(lr=0.0), dict(lr=-1.0), dict(beta1=0.0, beta2=0.0), dict(eps=0.0), dict(norm=1.0), dict(norm=float("inf"))):
+        assert check(**kw) == 0, kw
+    nan, inf = float("nan"), float("inf")
+    for kw in (dict(lr=nan), dict(lr=inf), dict(beta1=1.0), dict(beta2=1.0), dict(beta1=-0.1), dict(beta2=nan), dict(eps=-1.0),
+               dict(eps=1e-40), dict(eps=inf), dict(scale=0.0), dict(scale=-1.0), dict(scale=1e39), dict(scale=nan), dict(norm=-1.0),
+               dict(norm=nan)):
+        assert check(**kw) == BAD, kw
