@@ -112,7 +112,8 @@ ncclResult_t mscclAmdAdamWSetGrads(mscclAmdAdamW_t plan, const void* const* grad
  *   c = gradScale, and with a square sum and maxNorm > 0 times min(1, maxNorm / (norm + 1e-6)),
  *   norm = gradScale * sqrt(*gradSquareSum).
  * A square sum that is not finite leaves everything as it was, step included.
- * eps and gradScale are normal 32-bit values (eps may be 0), the betas in [0, 1).
+ * eps and gradScale are normal 32-bit values (eps may be 0), the betas in [0, 1) in 32
+ * bits too.
  *   lrDevice       NULL, or a 32-bit learning rate on the device in place of lr (a captured step
  *                  follows a schedule through it)
  *   gradSquareSum  NULL, or the square sum of the gradients as they are, over all ranks

@@ -283,6 +283,8 @@ ncclResult_t mscclAmdAdamWSetGrads(mscclAmdAdamW_t plan, const void* const* grad
 static ncclResult_t checkNumbers(const char* name, double lr, double beta1, double beta2, double eps, double gradScale, double maxNorm) {
   if (!std::isfinite(lr)) REFUSE("%s : lr is not finite", name);
   if (!(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1)) REFUSE("%s : betas (%g, %g) outside [0, 1)", name, beta1, beta2);
+  // (a moment that rounds to one times itself would only ever grow)
+  if ((float)beta1 == 1.f || (float)beta2 == 1.f) REFUSE("%s : betas (%.17g, %.17g) that are one in 32 bits", name, beta1, beta2);
   if (!(eps == 0 || (eps >= FLT_MIN && eps <= FLT_MAX))) REFUSE("%s : eps %g (0, or a normal 32-bit value)", name, eps);
   if (!(gradScale >= FLT_MIN && gradScale <= FLT_MAX)) REFUSE("%s : gradScale %g (a normal 32-bit value above zero)", name, gradScale);
   if (!(maxNorm >= 0)) REFUSE("%s : maxNorm %g", name, maxNorm);

@@ -235,3 +235,10 @@ def test_adamw_check_is_the_steps():
                dict(eps=1e-40), dict(eps=inf), dict(scale=0.0), dict(scale=-1.0), dict(scale=1e39), dict(scale=nan), dict(norm=-1.0),
                dict(norm=nan)):
         assert check(**kw) == BAD, kw
+
+
+@pytest.mark.parametrize("beta,rc", [(1 - 2.0 ** -24, 0), (1 - 2.0 ** -25, BAD), (1 - 1e-9, BAD), (1 - 1e-16, BAD)])
+def test_adamw_refuses_betas_that_are_one_in_32_bits(beta, rc):
+    L = ops._lib()
+    assert L.mscclAmdAdamWCheck(1e-3, beta, 0.999, 1e-8, 1.0, 0.0) == rc
+    assert L.mscclAmdAdamWCheck(1e-3, 0.9, beta, 1e-8, 1.0, 0.0) == rc
