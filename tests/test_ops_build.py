@@ -34,3 +34,27 @@ def test_objects_follow_their_flags(tmp_path):
         os.utime(x)
     assert out_of_date(build, "EXTRA_HIPFLAGS=-DANOTHER") == []
     assert out_of_date(build) == kernels   # and back
+
+
+def test_operators_kernels_have_no_scratch():
+    """They hold rows and chunks in registers: a spill would be a round trip through memory for each."""
+    kernels, name = {}, None
+    for f in glob.glob(os.path.join(ROOT, "build", "obj", "device", "ops_*.res")):
+        for line in open(f):
+            m = re.search(r"Function Name: (\S+)", line)
+            if m:
+                name = m.group(1)
+            m = re.search(r"(VGPRs|ScratchSize \[bytes/lane\]|LDS Size \[bytes/block\]): (\d+)", line)
+            if m and name:
+                kernels.setdefault(name, {}).setdefault(m.group(1).split()[0], int(m.group(2)))
+    if not kernels:
+        pytest.skip("no kernel resource reports (run __graft_entry__.build() first)")
+    families = ("adamwKernel", "adamwBeginKernel", "squareSumKernel", "sumPartialsKernel", "balanceStatsKernel",
+                "balanceFinishKernel", "balanceLossKernel", "balanceBackwardKernel", "tableWriteKernel", "gradWriteKernel")
+    for family in families:
+        assert any(family in k for k in kernels), family
+    for k, v in kernels.items():
+        assert v["ScratchSize"] == 0, (k, v)
+        assert v["LDS"] <= 65536, (k, v)   # what a launch takes without asking
+        # a workgroup of 1024 lanes has 128 registers a lane
+        assert v["VGPRs"] <= 128, (k, v)
