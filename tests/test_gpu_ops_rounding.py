@@ -92,14 +92,14 @@ def test_a_rounding_is_right_in_the_mean(param, grad, master, runs):
             assert bool((off.abs() <= step * far + near).all())
 
 
-def grads_ramp(t, steps, n):
+def grads_ramp(t, steps, n, noise=None):
     """One element of each run grows fivefold, the others stay."""
     g = torch.ones(n, device="cuda")
     g[::256] = 1.0 + 4.0 * min(1.0, 1.2 * t / steps)
     return g
 
 
-def grads_turn(t, steps, n, noise=gen(77)):
+def grads_turn(t, steps, n, noise):
     """Random gradients, of which a quarter falls to a quarter after a fifth of the steps and another rises fourfold."""
     size = torch.ones(256, device="cuda")
     if 5 * t > steps:
@@ -115,8 +115,9 @@ def test_averages_over_many_steps(grads, betas, steps):
     run's largest element the scale holds all digits."""
     n = 256 * 128
     k = Steps(n, BF16, F32, True)
+    noise = gen(77)
     for t in range(steps):
-        k.go(grads(t, steps, n), betas, lr=1e-6)
+        k.go(grads(t, steps, n, noise), betas, lr=1e-6)
     m, v = k.got()
     ratio = (v / k.v).reshape(-1, 256)
     for part in (slice(1, 64), slice(64, 128), slice(128, 256)):
