@@ -9,13 +9,13 @@
 // sums over rows stay in its registers too, then one exchange through LDS and one partial sum a
 // workgroup, which a second launch adds in a fixed order.  They are in 64 bits throughout and rounded once:
 // a router that starts from zero weights has equal rows, whose roundings in 32 bits do not average out
-// (a 64-bit FMA issues as a 32-bit one does; with the conversions it costs 0.45 us of the long batch's 21.2).
-// Counts are integers: their
-// atomics (in LDS) give the same result in any order.  The statistics' workgroups are large and
-// few, one a CU, so that there are few partial sums to add (256; with 512 the second launch takes 1 us
-// longer than the first gains); the row after the one that is worked on is always on its way.
-// 131072 tokens of 256 experts in bfloat16: statistics 17 to 18 us (68 MiB; reading and adding alone take 12.4)
-// and 3.4 for the second launch, gradient 23.4 us (128 MiB, 5.7 TB/s).
+// (a 64-bit FMA issues as a 32-bit one does; with the conversions the long batch takes 0.55 us more).
+// Counts are integers: their atomics (in LDS) give the same result in any order.  The statistics'
+// workgroups are large and few, one a CU, so that there are few partial sums to add (256; with 512 the
+// second launch takes 1 us longer than the first gains); the row after the one that is worked on is always
+// on its way.  131072 tokens of 256 experts in bfloat16: statistics 19.5 to 20.3 us (68 MiB, bound by
+// instruction issue: reading and adding in 32 bits alone take 12.4) and 2.8 to 3.9 for the second launch,
+// 21.65 for both and the loss in a stream of them; gradient 23.4 us (128 MiB, 5.7 TB/s).
 #include "ops.h"
 
 #include <type_traits>
