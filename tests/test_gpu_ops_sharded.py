@@ -68,3 +68,53 @@ def test_nothing_has_run_when_a_step_is_refused(monkeypatch):
         torch.cuda.synchronize()
         for c in comms:
             c.destroy()
+
+
+def test_a_sharded_run_with_8_bit_states():
+    """The documented chain (8-bit states rounded by chance, a 32-bit copy, clipping) against the same steps one
+    by one: the shards' plans alone, fed with what the collectives should bring."""
+    BF16 = torch.bfloat16
+    n, block, sizes = 2, 4352, [1000, 3, 517, 2049]
+    spans, at = [], 0
+    for k in sizes:
+        spans.append((at, k))
+        at += -(-k // 256) * 256
+    cut = lambda t: [t[a:a + k] for a, k in spans]  # noqa: E731
+    start = torch.randn(n * block, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(BF16)
+
+    def make(r, whole, shard):
+        p = cut(whole[r * block:(r + 1) * block])
+        w = [x.float() for x in p]
+        m, v, ms, vs = zip(*[ops.adamw_state(x, bits=8) for x in p])
+        step = torch.zeros(1, dtype=torch.int64, device="cuda")
+        plan = ops.AdamW(p, cut(shard), m, v, step, masters=w, exp_avg_scales=ms, exp_avg_sq_scales=vs, weight_decay=[0.1, 0.0, 0.1, 0.0],
+                         rounding="stochastic", seed=1)
+        return plan, ops.SquareSum(cut(shard)), [step, *w, *m, *v, *ms, *vs]
+    comms = M.Comm.init_all([0] * n)
+    try:
+        params = [start.clone() for _ in range(n)]
+        shards = [torch.zeros(block, dtype=BF16, device="cuda") for _ in range(n)]
+        plans, sums, states = (list(x) for x in zip(*[make(r, params[r], shards[r]) for r in range(n)]))
+        alone = start.clone()
+        parts = [torch.zeros(block, dtype=BF16, device="cuda") for _ in range(n)]
+        ours, ourSums, ourStates = (list(x) for x in zip(*[make(r, alone, parts[r]) for r in range(n)]))
+        for t in range(40):
+            grads = [(torch.randn(n * block, generator=torch.Generator(device="cuda").manual_seed(100 * t + r), device="cuda") * 3).to(BF16)
+                     for r in range(n)]
+            totals = ops.sharded_step(comms, grads, shards, params, plans, sums, lr=1e-3, betas=(0.9, 0.999), max_norm=1.0)
+            both = (grads[0].float() + grads[1].float()).to(BF16)   # added and rounded once
+            for r in range(n):
+                parts[r].copy_(both[r * block:(r + 1) * block])
+            total = ourSums[0]() + ourSums[1]()
+            assert all(torch.equal(x, total) for x in totals)
+            for p in ours:
+                p.step(1e-3, betas=(0.9, 0.999), grad_scale=0.5, grad_square_sum=total, max_norm=1.0)
+            torch.cuda.synchronize()
+            assert torch.equal(params[0], alone) and torch.equal(params[1], alone), t
+            for a, b in zip(states, ourStates):
+                assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a, b)), t
+        assert not torch.equal(alone, start)
+    finally:
+        torch.cuda.synchronize()
+        for c in comms:
+            c.destroy()
