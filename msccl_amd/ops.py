@@ -112,7 +112,11 @@ def _changed(tensors) -> None:
 
 def _versions(tensors):
     """One of these for each version counter (views share their base's)."""
-    return list({id(t if t._base is None else t._base): t for t in tensors}.values())
+    seen = {}
+    for t in tensors:
+        base = t if t._base is None else t._base
+        seen.setdefault(id(base), (t, base))   # (held: a number may be another's once its object is gone)
+    return [t for t, _ in seen.values()]
 
 
 class _Plan:
@@ -335,7 +339,7 @@ class AdamW(_Plan):
                 g.record_stream(s)
         with torch.cuda.device(self.device):
             captured = torch.cuda.is_current_stream_capturing()
-        if captured:   # until a replay the table holds the earlier ones, and a later call does not end the replays
+        if captured:   # until a replay the table holds the earlier ones, and every replay sets these again
             self._captured.append((self.tensors[1], list(grads)))
         self.tensors[1] = list(grads)
         self.grad_span = _span(grads)

@@ -242,3 +242,15 @@ def test_adamw_refuses_betas_that_are_one_in_32_bits(beta, rc):
     L = ops._lib()
     assert L.mscclAmdAdamWCheck(1e-3, beta, 0.999, 1e-8, 1.0, 0.0) == rc
     assert L.mscclAmdAdamWCheck(1e-3, 0.9, beta, 1e-8, 1.0, 0.0) == rc
+
+
+def test_one_tensor_for_each_version_counter():
+    flats = [torch.zeros(16) for _ in range(200)]
+    views = [f[4 * i:4 * i + 4] for f in flats for i in range(3)]
+    whole = [torch.zeros(3) for _ in range(5)]
+    del flats   # (the views keep their bases)
+    got = ops._versions(views + whole + whole)
+    assert len(got) == 205
+    before = [t._version for t in views + whole]
+    ops._changed(got)
+    assert [t._version for t in views + whole] == [v + 1 for v in before]
