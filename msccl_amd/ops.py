@@ -344,6 +344,14 @@ class AdamW(_Plan):
         self.tensors[1] = list(grads)
         self.grad_span = _span(grads)
 
+    def _say(self, betas, level) -> None:
+        """The warning of a plan that was told no rounding, once."""
+        if betas[1] > 0.9375:   # a root of v decays by 1 - sqrt(beta2), half a code's step is 2^-5 or more
+            self._unsaid = False
+            warnings.warn("AdamW: second moments of 8 bits that are rounded to nearest drift over many steps with beta2 %g; "
+                          "rounding=\"stochastic\" follows them (rounding=\"nearest\" says that this is meant)" % betas[1],
+                          stacklevel=level)
+
     def _check_step(self, lr, betas, eps, grad_scale, max_norm) -> None:
         """What step and the library refuse, without a step."""
         if not self.handle:
@@ -354,6 +362,8 @@ class AdamW(_Plan):
         if max_norm is not None and not max_norm > 0:
             raise ValueError("max_norm must be above zero")
         _check(_lib().mscclAmdAdamWCheck(lr, betas[0], betas[1], eps, grad_scale, max_norm or 0.0), "mscclAmdAdamWCheck")
+        if self._unsaid:   # (here, where a warning that is an error stops no collective)
+            self._say(betas, 4)
 
     def step(self, lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8, grad_scale: float = 1.0,
              grad_square_sum: Optional[torch.Tensor] = None, max_norm: Optional[float] = None) -> None:
@@ -372,11 +382,8 @@ class AdamW(_Plan):
             total = grad_square_sum.data_ptr()
         if max_norm is not None and not max_norm > 0:
             raise ValueError("max_norm must be above zero")
-        if self._unsaid and betas[1] > 0.9375:   # a root of v decays by 1 - sqrt(beta2), half a code's step is 2^-5 or more
-            self._unsaid = False
-            warnings.warn("AdamW: second moments of 8 bits that are rounded to nearest drift over many steps with beta2 %g; "
-                          "rounding=\"stochastic\" follows them (rounding=\"nearest\" says that this is meant)" % betas[1],
-                          stacklevel=2)
+        if self._unsaid:
+            self._say(betas, 3)
         launch, args = _lib().mscclAmdAdamWStep, (self.handle, lr, at, betas[0], betas[1], eps, grad_scale, total,
                                                   max_norm or 0.0, stream)
         if _elsewhere(self.device):

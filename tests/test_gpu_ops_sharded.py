@@ -118,3 +118,32 @@ def test_a_sharded_run_with_8_bit_states():
         torch.cuda.synchronize()
         for c in comms:
             c.destroy()
+
+
+def test_a_warning_that_is_an_error_comes_before_the_collectives(monkeypatch):
+    import warnings
+    comms = M.Comm.init_all([0, 0])
+    try:
+        k = Ranks(comms)
+        plans = []
+        for r in range(2):
+            p = k.params[r][r * 512:(r + 1) * 512]
+            m, v, ms, vs = ops.adamw_state(p, bits=8)
+            k.state += [m, v, ms, vs]
+            step = torch.zeros(1, dtype=torch.int64, device="cuda")
+            plans.append(ops.AdamW([p], [k.shards[r]], [m], [v], step, exp_avg_scales=[ms], exp_avg_sq_scales=[vs]))
+        called, real = [], M.Comm.reduce_scatter
+        monkeypatch.setattr(M.Comm, "reduce_scatter", lambda *a, **kw: (called.append(1), real(*a, **kw))[1])
+        with warnings.catch_warnings():
+            warnings.simplefilter("error")
+            for _ in range(2):   # each of the plans says it once
+                with pytest.raises(UserWarning):
+                    k.go(plans=plans)
+                assert called == []
+            k.go(plans=plans)
+        assert len(called) == 2
+        torch.cuda.synchronize()
+    finally:
+        torch.cuda.synchronize()
+        for c in comms:
+            c.destroy()
