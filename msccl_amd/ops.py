@@ -590,7 +590,8 @@ def balance_backward(logits: torch.Tensor, counts: torch.Tensor, top_k: int, coe
                      score: str = "softmax", out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """The gradient of balance_loss at these logits (counts: the loss's own, over all ranks; they carry no
     gradient), in the type of logits; padded rows get zeros.  grad_output: the loss's own gradient, float32
-    of one element.  out: where to write it; accumulate: it is added to what `out` holds."""
+    of one element.  out: where to write it (logits itself, or no element of theirs); accumulate: it is added
+    to what `out` holds, which is not logits then."""
     r = _router(logits, None, top_k, valid, score)
     dev = logits.device
     t, e = logits.shape
